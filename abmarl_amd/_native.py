@@ -127,7 +127,84 @@ def build(force=False, verbose=False, stamps=False, checks=False, out=None, extr
     return out
 
 
+LEARN_SRCS = [os.path.join(PKG, 'csrc', f) for f in ('gw_policy.hip', 'gw_recurrence.hip')]
+LEARN_DEPS = LEARN_SRCS + [os.path.join(PKG, 'csrc', 'gw_learn.hpp'), INCLUDE,
+                           os.path.join(os.path.dirname(PKG), 'include', 'gw_learn.h')]
+LIB_LEARN = os.path.join(PKG, '_build', 'libgw_learn.so')
+
+# every entry point declared in include/gw_learn.h
+_i64, _f32 = C.c_int64, C.c_float
+LEARN_SIGNATURES = {
+    'gw_policy_sample': (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
+    'gw_policy_loss_workspace': (_i64, [_i64]),
+    'gw_policy_loss': (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64,
+                              _f32, _f32, _f32, _f32, _f32, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    'gw_recurrence_workspace': (_i64, [_i64, _i64]),
+    'gw_recurrence': (_i32, [_i32, _i32, _i64, _i64, _vp, _vp, _i64, _f32, _vp, _i64, _vp, _i32,
+                             _vp, _vp, _vp, _vp, _i64, _vp]),
+    'gw_recurrence_backward_workspace': (_i64, [_i64, _i64, _i64]),
+    'gw_recurrence_backward': (_i32, [_i32, _i32, _i64, _i64, _vp, _vp, _i64, _f32, _vp, _i64, _vp, _i32,
+                                      _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    'gw_fragment_marks': (_i32, [_i64, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp]),
+    'gw_advantages': (_i32, [_i32, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _f32,
+                             _vp, _vp, _vp, _vp, _i64, _vp]),
+    'gw_learn_last_error': (C.c_char_p, []),
+    'gw_learn_abi_version': (_i32, []),
+}
+
+
+def build_learn(force=False, verbose=False, out=None, extra_flags=()):
+    """Compile the policy operators (libgw_learn.so) for gfx950, one object a
+    source, in parallel.  Their float code is built without packed-fp32
+    instructions and with contraction (fma) allowed; the engine's own is not:
+    it has numpy's roundings to meet."""
+    out = out or LIB_LEARN
+    if not force and os.path.exists(out) and \
+            os.path.getmtime(out) >= max(os.path.getmtime(d) for d in LEARN_DEPS):
+        return out
+    objdir = os.path.join(os.path.dirname(out), 'obj_' + os.path.splitext(os.path.basename(out))[0])
+    os.makedirs(objdir, exist_ok=True)
+    objs = [os.path.join(objdir, os.path.basename(s)[:-4] + '.o') for s in LEARN_SRCS]
+    cmds = [[HIPCC, f'--offload-arch={ARCH}', '-O3', '-std=c++17', '-fPIC', '-Wno-unused-result',
+             '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops'] + list(extra_flags) +
+            ['-c', '-o', o, s] for s, o in zip(LEARN_SRCS, objs)]
+    link = [HIPCC, f'--offload-arch={ARCH}', '-shared', '-fPIC', '-o', out + '.tmp'] + objs
+    if verbose:
+        for c in cmds + [link]:
+            print(' '.join(c))
+    procs = [subprocess.Popen(c) for c in cmds]
+    failed = [' '.join(c) for c, p in zip(cmds, procs) if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    subprocess.check_call(link)
+    os.replace(out + '.tmp', out)
+    return out
+
+
 _lib = None
+_learn = None
+
+
+def learn_lib():
+    """The loaded library of the policy operators; raises if it is missing (no fallback)."""
+    global _learn
+    if _learn is None:
+        if not os.path.exists(LIB_LEARN):
+            raise RuntimeError(f"HIP library {LIB_LEARN} is missing; run "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`")
+        L = C.CDLL(LIB_LEARN)
+        for name, (res, args) in LEARN_SIGNATURES.items():
+            fn = getattr(L, name)
+            fn.restype = res
+            fn.argtypes = args
+        _learn = L
+    return _learn
+
+
+def check_learn(status, what):
+    if status != 0:
+        msg = learn_lib().gw_learn_last_error().decode(errors='replace')
+        raise EngineError(f"{what} failed with status {status}: {msg}")
 
 
 def lib():
