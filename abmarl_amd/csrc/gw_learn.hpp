@@ -39,6 +39,13 @@ constexpr float NEG_INF = -__builtin_inff();
 // the larger of two, NaN if either is: a NaN logit must not vanish in a maximum
 __device__ inline float max_nan(float a, float b) { return (b > a || b != b) ? b : a; }
 
+// what a wave's lanes have written to LDS is there for its other lanes
+__device__ inline void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 template <class V>
 __device__ inline V wave_sum(V v)
 {

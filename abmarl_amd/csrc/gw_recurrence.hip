@@ -9,8 +9,10 @@ constexpr int SEG = GW_RECURRENCE_SEGMENT;
 
 struct RecurArgs {
     int64_t T, n;
-    const void* x; const void* gate; int64_t gate_span; float gate_value;
-    const uint8_t* cut; int64_t cut_span;
+    const void* x; const void* gate; const uint8_t* cut;
+    uint32_t gate_span, cut_span;                // channels per gate, per cut
+    int64_t gates, cuts;                         // of a step
+    float gate_value;
     const float* state; int32_t reverse;
     void* h; float* last; float* carry;          // forward
     const void* dh; const float* dlast;          // backward
@@ -18,87 +20,349 @@ struct RecurArgs {
     float* part; int32_t parts;                  // [T][n / gate_span][parts]: shared gates' gradients
 };
 
+// ------------------------------------------------------------------ the scan
+// A step is the map h -> a h + b; maps compose, so the steps can be split.  A
+// wave holds 64 neighbouring channels (one a lane) and SEG steps of them in
+// registers.  NW waves of a workgroup hold NW such segments in time, exchange
+// their maps through LDS and walk their own steps from the state that reaches
+// them: one pass over the data.  CW waves stand side by side in channels.
+// Where channels and waves do not fill the device, the steps are cut into
+// chunks too: a first launch makes every chunk's map (reading gates and
+// values), a second composes the maps before its own and walks.
+
+struct Map { float a, b; };
+
+// A map drops the state only where a gate is 0.  The product of others may
+// underflow: then the smallest number keeps an infinite state infinite.
+__device__ inline float keep(float a, bool zero) { return zero ? 0.f : (a == 0.f ? 1.4e-45f : a); }
+
+// a h + b, where a = 0 drops any state (0 * inf would be NaN)
+__device__ inline float advance(float a, float h, float b) { return fmaf(a, a == 0.f ? 0.f : h, b); }
+
+// the same for a segment's map, whose product of gates may have overflowed
+__device__ inline float apply(Map m, float h) { return m.a == 0.f || h == 0.f ? m.b : fmaf(m.a, h, m.b); }
+
+__device__ inline Map compose(Map first, Map then)
+{
+    return Map{keep(first.a * then.a, first.a == 0.f || then.a == 0.f), apply(then, first.b)};
+}
+
+// chunks of the steps; maps[chunk][n]
+struct Chunks { int32_t count; int64_t steps; float2* maps; };
+
+// The state that reaches wave w's segment, from the one that reaches the
+// tile (`in`, which becomes the one behind the tile) and the waves' maps.
+template <int NW>
+__device__ inline float join(float2 (*box)[WAVE], int w, int lane, Map m, float& in)
+{
+    box[w][lane] = make_float2(m.a, m.b);
+    __syncthreads();
+    float h = in, mine = in;
+#pragma unroll
+    for (int v = 0; v < NW; v++) {
+        mine = v == w ? h : mine;
+        const float2 q = box[v][lane];
+        h = apply(Map{q.x, q.y}, h);
+    }
+    in = h;
+    return mine;
+}
+
+// The state that reaches a chunk: `state` through the maps of the chunks
+// before it, shared out to the NW waves.
+template <int NW>
+__device__ inline float reach_chunk(float2 (*box)[WAVE], const Chunks& s, int64_t n, int64_t c, int w, int lane,
+                                    float state)
+{
+    const int chunk = blockIdx.y;
+    if (chunk == 0) return state;
+    const int per = (chunk + NW - 1) / NW, from = w * per, to = from + per < chunk ? from + per : chunk;
+    Map m{1.f, 0.f};
+    for (int j = from; j < to; j += 8) {
+        float2 q[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) q[k] = s.maps[(int64_t)(j + k < to ? j + k : to - 1) * n + c];
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (j + k < to) m = compose(m, Map{q[k].x, q[k].y});
+    }
+    if constexpr (NW == 1) return apply(m, state);
+    join<NW>(box, w, lane, m, state);
+    __syncthreads();
+    return state;
+}
+
+// Where a wave stands: channels from c0 (uniform), lane l of them (a valid
+// one where the lane is not `on`), time segment w of NW.
+struct Place {
+    int64_t c0;
+    int w, lane;
+    uint32_t l;
+    bool on;
+    __device__ int64_t c() const { return c0 + l; }
+};
+
+template <int NW, int CW>
+__device__ inline Place place(int64_t n)
+{
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    Place p;
+    p.lane = threadIdx.x & 63;
+    p.w = NW == 1 ? 0 : wave;
+    p.c0 = ((int64_t)blockIdx.x * CW + (NW == 1 ? wave : 0)) * WAVE;
+    const int64_t left = n - 1 - p.c0;
+    p.on = p.lane <= left;
+    p.l = p.on ? p.lane : 0;
+    return p;
+}
+
+// A row of one value per `span` channels as the wave's channels see it: from
+// a uniform place, per lane a small offset
+struct Shared {
+    uint32_t first, l;
+    __device__ Shared(uint32_t span, const Place& p)
+    {
+        // (fewer than 2^31 channels)
+        first = (uint32_t)p.c0 / span;
+        l = (((uint32_t)p.c0 + p.l) / span - first) & 63u;
+    }
+};
+
 // step i of the recurrence's own order is step at(i) of the slabs
 __device__ inline int64_t step_at(const RecurArgs& a, int64_t i) { return a.reverse ? a.T - 1 - i : i; }
 
-template <class TG>
-__device__ inline float gate_at(const RecurArgs& a, int64_t t, int64_t c)
+// SEG rows of `stride` values from step i0 on, one value a lane: f(k, value).
+// Whole segments are one run of loads; in the last one the steps that are
+// there are a uniform branch each.
+template <class V, class F>
+__device__ inline void load_rows(const RecurArgs& a, const V* slab, int64_t stride, int64_t i0, int64_t first,
+                                 uint32_t l, F f)
 {
-    if (a.cut && a.cut[t * (a.n / a.cut_span) + c / a.cut_span]) return 0.f;
-    return a.gate ? (float)((const TG*)a.gate)[t * (a.n / a.gate_span) + c / a.gate_span] : a.gate_value;
-}
-
-// a cut step's state is not used at all: 0 * inf would be NaN
-__device__ inline float advance(float gate, float h, float x) { return (gate == 0.f ? 0.f : gate * h) + x; }
-
-// One thread per channel, the steps one after another.
-template <class T, class TG>
-__global__ __launch_bounds__(256) void recur_kernel(RecurArgs a)
-{
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= a.n) return;
-    float h = a.state ? a.state[c] : 0.f;
-    for (int64_t i = 0; i < a.T; i++) {
-        const int64_t t = step_at(a, i);
-        if (a.carry && i % SEG == 0) a.carry[i / SEG * a.n + c] = h;
-        h = advance(gate_at<TG>(a, t, c), h, (float)((const T*)a.x)[t * a.n + c]);
-        ((T*)a.h)[t * a.n + c] = (T)h;
+    const V* row = slab + step_at(a, i0) * stride + first;
+    const int64_t next = a.reverse ? -stride : stride;
+    V v[SEG];
+    if (i0 + SEG <= a.T) {
+#pragma unroll
+        for (int k = 0; k < SEG; k++, row += next) v[k] = row[l];
+#pragma unroll
+        for (int k = 0; k < SEG; k++) f(k, v[k]);
+    } else {
+        const int m = (int)(a.T - i0);
+#pragma unroll
+        for (int k = 0; k < SEG; k++, row += next)
+            if (k < m) f(k, row[l]);
     }
-    if (a.last) a.last[c] = h;
 }
 
-// One thread per channel; the segments from the last to the first: the state
-// before each step again from the segment's carry, then the steps backwards.
-template <class T, class TG>
-__global__ __launch_bounds__(64) void recur_backward_kernel(RecurArgs a)
+// The gates of SEG steps from i0 (0 where cut; 1 behind the last step), and
+// cuts as bits
+template <class TG>
+__device__ inline uint32_t load_gates(const RecurArgs& a, int64_t i0, const Shared& g, const Shared& c, float* gate)
 {
-    // a wave holds channels of one gate only, so its sum is one gate's part
-    // (a gate of its own for each channel: all of them are one group)
-    const int64_t span = a.gate_span == 1 ? a.n : a.gate_span;
-    const int64_t per = (span + 63) / 64;
-    const int64_t group = blockIdx.x / per, piece = blockIdx.x % per;
-    const int64_t in = piece * 64 + threadIdx.x;
-    const bool on = in < span;
-    const int64_t c = group * span + (on ? in : 0);
-    float into = on && a.dlast ? a.dlast[c] : 0.f;       // what the next step hands back
-    for (int64_t s = (a.T + SEG - 1) / SEG; s-- > 0;) {
-        const int64_t i0 = s * SEG;
-        const int m = a.T - i0 < SEG ? (int)(a.T - i0) : SEG;
-        float before[SEG];
-        float h = a.carry[s * a.n + c];
-        for (int k = 0; k < m; k++) {
-            const int64_t t = step_at(a, i0 + k);
-            before[k] = h;
-            h = advance(gate_at<TG>(a, t, c), h, (float)((const T*)a.x)[t * a.n + c]);
+    uint32_t bits = 0;
+    const int m = i0 + SEG <= a.T ? SEG : (int)(a.T - i0);
+#pragma unroll
+    for (int k = 0; k < SEG; k++) gate[k] = k < m ? a.gate_value : 1.f;
+    if (a.gate) load_rows(a, (const TG*)a.gate, a.gates, i0, g.first, g.l, [&](int k, TG v) { gate[k] = (float)v; });
+    if (a.cut)
+        load_rows(a, a.cut, a.cuts, i0, c.first, c.l, [&](int k, uint8_t v) {
+            bits |= (v ? 1u : 0u) << k;
+            gate[k] = v ? 0.f : gate[k];
+        });
+    return bits;
+}
+
+// SEG steps of a slab like x; 0 behind the last step
+template <class T>
+__device__ inline void load_values(const RecurArgs& a, const void* slab, int64_t i0, const Place& p, float* v)
+{
+#pragma unroll
+    for (int k = 0; k < SEG; k++) v[k] = 0.f;
+    load_rows(a, (const T*)slab, a.n, i0, p.c0, p.l, [&](int k, T x) { v[k] = (float)x; });
+}
+
+// The map of a segment: forwards h -> gate h + x, or (BACK) from the last step
+// to the first into -> gate (into + dh)
+template <bool BACK>
+__device__ inline Map segment_map(const float* gate, const float* v)
+{
+    Map m{1.f, 0.f};
+    bool zero = false;
+#pragma unroll
+    for (int i = 0; i < SEG; i++) {
+        const int k = BACK ? SEG - 1 - i : i;
+        m.b = BACK ? advance(gate[k], m.b + v[k], 0.f) : advance(gate[k], m.b, v[k]);
+        m.a *= gate[k];
+        zero |= gate[k] == 0.f;
+    }
+    m.a = keep(m.a, zero);
+    return m;
+}
+
+// Every chunk's map; wave w takes its share of the chunk's segments.  BACK:
+// the gradient's, chunks and segments counted from the last.
+template <class T, class TG, int NW, bool BACK>
+__global__ __launch_bounds__(64 * NW) void maps_kernel(RecurArgs a, Chunks s)
+{
+    __shared__ float2 box[NW][WAVE];
+    const Place p = place<NW, 1>(a.n);
+    const Shared g(a.gate_span, p), c(a.cut_span, p);
+    const int64_t from = blockIdx.y * s.steps + p.w * (s.steps / NW), segs = (a.T + SEG - 1) / SEG;
+    Map m{1.f, 0.f};
+    for (int64_t i = from; i < from + s.steps / NW; i += SEG) {
+        if (i >= segs * SEG) break;
+        const int64_t i0 = BACK ? (segs - 1) * SEG - i : i;
+        float gate[SEG], v[SEG];
+        load_gates<TG>(a, i0, g, c, gate);
+        if (BACK && !a.dh) {
+#pragma unroll
+            for (int k = 0; k < SEG; k++) v[k] = 0.f;
+        } else load_values<T>(a, BACK ? a.dh : a.x, i0, p, v);
+        m = compose(m, segment_map<BACK>(gate, v));
+    }
+    box[p.w][p.lane] = make_float2(m.a, m.b);
+    __syncthreads();
+    if (p.w != 0) return;
+    for (int v = 1; v < NW; v++) m = compose(m, Map{box[v][p.lane].x, box[v][p.lane].y});
+    if (p.on) s.maps[blockIdx.y * a.n + p.c()] = make_float2(m.a, m.b);
+}
+
+template <class T, class TG, int NW, int CW>
+__global__ __launch_bounds__(64 * NW * CW) void recur_kernel(RecurArgs a, Chunks s)
+{
+    __shared__ float2 box[2][NW][WAVE];
+    const Place p = place<NW, CW>(a.n);
+    if (NW == 1 && p.c0 >= a.n) return;
+    const Shared g(a.gate_span, p), c(a.cut_span, p);
+    const int64_t from = blockIdx.y * s.steps, to = from + s.steps < a.T ? from + s.steps : a.T;
+    float in = reach_chunk<NW>(box[0], s, a.n, p.c(), p.w, p.lane, a.state ? a.state[p.c()] : 0.f);
+    int turn = 0;
+    for (int64_t i = from; i < to; i += NW * SEG) {
+        const int64_t i0 = i + p.w * SEG;
+        const bool there = i0 < a.T;
+        float gate[SEG], x[SEG];
+        if (there) {
+            load_gates<TG>(a, i0, g, c, gate);
+            load_values<T>(a, a.x, i0, p, x);
         }
-        for (int k = m - 1; k >= 0; k--) {
-            const int64_t t = step_at(a, i0 + k);
-            const float g = into + (a.dh ? (float)((const T*)a.dh)[t * a.n + c] : 0.f);
-            const float gate = gate_at<TG>(a, t, c);
-            into = gate == 0.f ? 0.f : gate * g;
-            if (on) ((T*)a.dx)[t * a.n + c] = (T)g;
-            if (!a.dgate) continue;
-            const bool cut = a.cut && a.cut[t * (a.n / a.cut_span) + c / a.cut_span];
-            float d = cut || !on ? 0.f : g * before[k];
-            if (a.gate_span == 1) {
-                if (on) ((TG*)a.dgate)[t * a.n + c] = (TG)d;
-            } else {
-                d = wave_sum(d);
-                if (threadIdx.x == 0) a.part[(t * (a.n / a.gate_span) + group) * a.parts + piece] = d;
+        float h = in;
+        if constexpr (NW > 1)
+            h = join<NW>(box[turn], p.w, p.lane, there ? segment_map<false>(gate, x) : Map{1.f, 0.f}, in);
+        turn ^= 1;
+        if (!there) continue;
+        if (p.on && a.carry) a.carry[i0 / SEG * a.n + p.c()] = h;
+        const int m = i0 + SEG <= a.T ? SEG : (int)(a.T - i0);
+        T* row = (T*)a.h + step_at(a, i0) * a.n + p.c0;
+        const int64_t next = a.reverse ? -a.n : a.n;
+#pragma unroll
+        for (int k = 0; k < SEG; k++, row += next) {
+            h = advance(gate[k], h, x[k]);
+            if (k < m && p.on) row[p.l] = (T)h;
+        }
+        if constexpr (NW == 1) in = h;
+    }
+    if (a.last && p.on && p.w == 0 && to == a.T) a.last[p.c()] = in;
+}
+
+// The sums over the channels that share a gate, of one segment's products
+// d[k] (one a lane): a gate's channels lie side by side, so a wave holds a
+// few whole gates and parts of two.  d crosses LDS; then every lane adds the
+// channels of (step, gate) pairs, in their order.
+template <class TG>
+__device__ inline void gate_sums(const RecurArgs& a, float (*tile)[WAVE + 1], int64_t i0, const Place& p, const float* d)
+{
+#pragma unroll
+    for (int k = 0; k < SEG; k++) tile[k][p.lane] = p.on ? d[k] : 0.f;
+    wave_sync();
+    const int64_t first = (uint32_t)p.c0 / a.gate_span, wave = p.c0 / WAVE;
+    const int64_t end = p.c0 + WAVE < a.n ? p.c0 + WAVE : a.n;
+    const int gates = (int)((uint32_t)(end - 1) / a.gate_span - first) + 1;
+    for (int q = p.lane; q < gates * SEG; q += WAVE) {
+        const int64_t gate = first + q / SEG;
+        const int k = q % SEG;
+        if (i0 + k >= a.T) continue;
+        const int64_t lo = gate * a.gate_span - p.c0, hi = lo + a.gate_span;
+        float sum = 0.f;
+        for (int j = lo > 0 ? (int)lo : 0; j < (hi < WAVE ? (int)hi : WAVE); j++) sum += tile[k][j];
+        const int64_t at = step_at(a, i0 + k) * a.gates + gate;
+        if (a.parts == 1) ((TG*)a.dgate)[at] = (TG)sum;
+        else a.part[at * a.parts + (int)(wave - gate * a.gate_span / WAVE)] = sum;
+    }
+    wave_sync();
+}
+
+// The segments from the last to the first: the states before a segment's
+// steps again from its carry, the gradient that reaches it as the forward
+// pass joins states, then its steps backwards.
+template <class T, class TG, int NW, int CW, bool SUMS>
+__global__ __launch_bounds__(64 * NW * CW) void recur_backward_kernel(RecurArgs a, Chunks s)
+{
+    __shared__ float2 box[2][NW][WAVE];
+    __shared__ float tiles[SUMS ? NW * CW : 1][SEG][WAVE + 1];
+    const Place p = place<NW, CW>(a.n);
+    if (NW == 1 && p.c0 >= a.n) return;
+    const Shared g(a.gate_span, p), c(a.cut_span, p);
+    const int64_t segs = (a.T + SEG - 1) / SEG;
+    const int64_t from = blockIdx.y * s.steps, to = from + s.steps < segs * SEG ? from + s.steps : segs * SEG;
+    float in = reach_chunk<NW>(box[0], s, a.n, p.c(), p.w, p.lane, a.dlast ? a.dlast[p.c()] : 0.f);
+    int turn = 0;
+    for (int64_t i = from; i < to; i += NW * SEG) {
+        // counted from the last segment; a wave whose place lies before the first has nothing to do
+        const int64_t i0 = (segs - 1) * SEG - (i + p.w * SEG);
+        const bool there = i0 >= 0;
+        float gate[SEG], before[SEG], dh[SEG];
+        uint32_t cut = 0;
+        if (there) {
+            float x[SEG];
+            cut = load_gates<TG>(a, i0, g, c, gate);
+            load_values<T>(a, a.x, i0, p, x);
+            if (a.dh) load_values<T>(a, a.dh, i0, p, dh);
+            else {
+#pragma unroll
+                for (int k = 0; k < SEG; k++) dh[k] = 0.f;
+            }
+            float h = a.carry[i0 / SEG * a.n + p.c()];
+#pragma unroll
+            for (int k = 0; k < SEG; k++) {
+                before[k] = h;
+                h = advance(gate[k], h, x[k]);
             }
         }
+        float into = in;
+        if constexpr (NW > 1)
+            into = join<NW>(box[turn], p.w, p.lane, there ? segment_map<true>(gate, dh) : Map{1.f, 0.f}, in);
+        if (there) {
+            const int m = i0 + SEG <= a.T ? SEG : (int)(a.T - i0);
+            const int64_t next = a.reverse ? -a.n : a.n, at = step_at(a, i0 + SEG - 1) * a.n + p.c0;
+            T* row = (T*)a.dx + at;
+            TG* gate_row = (TG*)a.dgate + at;
+#pragma unroll
+            for (int k = SEG - 1; k >= 0; k--, row -= next, gate_row -= next) {
+                const float gk = into + dh[k];
+                if (k < m && p.on) row[p.l] = (T)gk;
+                into = advance(gate[k], gk, 0.f);
+                dh[k] = (cut >> k & 1) ? 0.f : gk * before[k];
+                if (!SUMS && a.dgate && k < m && p.on) gate_row[p.l] = (TG)dh[k];
+            }
+            if constexpr (SUMS) gate_sums<TG>(a, tiles[NW == 1 ? (int)threadIdx.x >> 6 : p.w], i0, p, dh);
+        }
+        if constexpr (NW == 1) in = into;
+        turn ^= 1;
     }
-    if (on && a.dstate) a.dstate[c] = into;
+    if (a.dstate && p.on && p.w == 0 && to == segs * SEG) a.dstate[p.c()] = in;
 }
 
+// the waves' parts of every shared gate's sum, in their order
 template <class TG>
-__global__ __launch_bounds__(256) void gate_parts_kernel(const float* part, int parts, int64_t gates, TG* dgate)
+__global__ __launch_bounds__(256) void gate_parts_kernel(RecurArgs a)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= gates) return;
+    const int64_t gates = a.gates, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.T * gates) return;
+    const int64_t lo = i % gates * a.gate_span;
+    const int pieces = (int)((lo + a.gate_span - 1) / WAVE - lo / WAVE) + 1;
     float s = 0.f;
-    for (int p = 0; p < parts; p++) s += part[i * parts + p];
-    dgate[i] = (TG)s;
+    for (int p = 0; p < pieces; p++) s += a.part[i * a.parts + p];
+    ((TG*)a.dgate)[i] = (TG)s;
 }
 
 __global__ __launch_bounds__(256) void marks_kernel(int64_t T, int64_t E, const uint8_t* all_done,
@@ -136,62 +400,170 @@ struct AdvArgs {
     float* advantage; float* target; uint8_t* valid;
 };
 
-// whether the lane acted in step t
-__device__ inline bool acted(const AdvArgs& a, int64_t t, int64_t c, int64_t e, uint8_t mark)
+// One segment of a lane's steps: for each step the map carry -> gate carry +
+// delta, the value (0 where the lane did not act) and whether it acted.
+template <class TR, class TV>
+__device__ inline uint32_t load_steps(const AdvArgs& a, int64_t n, int64_t i0, const Place& p, const Shared& env,
+                                      bool acts, float* gate, float* delta, float* value)
 {
-    if (mark & (GW_MARK_RESET | GW_MARK_SKIP)) return false;
-    if (a.acts && !a.acts[c % a.A]) return false;
-    if (t == 0) return a.live[c] != 0;
-    return (a.marks[(t - 1) * a.E + e] & GW_MARK_END) || !a.done[(t - 1) * a.E * a.A + c];
+    uint8_t done[SEG + 1], mark[SEG + 1];       // [k]: of the step before step k
+    float next[SEG + 1];
+#pragma unroll
+    for (int k = 0; k <= SEG; k++) {
+        const int64_t t = i0 + k <= a.T ? i0 + k : a.T, b = t > 0 ? t - 1 : 0;
+        done[k] = (a.done + b * n + p.c0)[p.l];
+        mark[k] = (a.marks + b * a.E + env.first)[env.l];
+        next[k] = (float)((const TV*)a.value + t * n + p.c0)[p.l];
+    }
+#pragma unroll
+    for (int k = 0; k < SEG; k++)
+        delta[k] = (float)((const TR*)a.reward + (i0 + k < a.T ? i0 + k : a.T - 1) * n + p.c0)[p.l];
+    const bool live = i0 > 0 || (a.live + p.c0)[p.l];
+    uint32_t bits = 0;
+#pragma unroll
+    for (int k = 0; k < SEG; k++) {
+        const uint8_t m = mark[k + 1];
+        const bool before = i0 + k == 0 ? live : (mark[k] & GW_MARK_END) || !done[k];
+        const bool ok = acts && before && !(m & (GW_MARK_RESET | GW_MARK_SKIP)) && i0 + k < a.T;
+        const bool final = done[k + 1] || (m & GW_MARK_END);
+        const float d = delta[k] - next[k] + (final ? 0.f : a.gamma * next[k + 1]);
+        delta[k] = ok ? d : 0.f;
+        value[k] = ok ? next[k] : 0.f;
+        gate[k] = i0 + k >= a.T ? 1.f : ok && !final && !(m & GW_MARK_TRUNCATED) ? a.gamma * a.lam : 0.f;
+        bits |= (ok ? 1u : 0u) << k;
+    }
+    return bits;
+}
+
+// The recurrence from the last step to the first, split as the gradient's
+// (MAPS: the chunks' maps only).
+template <class TR, class TV, int NW, int CW, bool MAPS>
+__global__ __launch_bounds__(64 * NW * CW) void advantages_kernel(AdvArgs a, Chunks s)
+{
+    __shared__ float2 box[2][NW][WAVE];
+    const int64_t n = a.E * a.A;
+    const Place p = place<NW, CW>(n);
+    if (NW == 1 && p.c0 >= n) return;
+    const Shared env((uint32_t)a.A, p);
+    const bool acts = !a.acts || a.acts[(uint32_t)p.c() % (uint32_t)a.A];
+    const int64_t segs = (a.T + SEG - 1) / SEG;
+    const int64_t from = blockIdx.y * s.steps, to = from + s.steps < segs * SEG ? from + s.steps : segs * SEG;
+    float in = 0.f;
+    Map whole{1.f, 0.f};
+    if (!MAPS) in = reach_chunk<NW>(box[0], s, n, p.c(), p.w, p.lane, 0.f);
+    int turn = 0;
+    for (int64_t i = from; i < to; i += NW * SEG) {
+        const int64_t i0 = (segs - 1) * SEG - (i + p.w * SEG);
+        const bool there = i0 >= 0;
+        float gate[SEG], delta[SEG], value[SEG];
+        uint32_t ok = 0;
+        Map m{1.f, 0.f};
+        if (there) {
+            ok = load_steps<TR, TV>(a, n, i0, p, env, acts, gate, delta, value);
+            bool zero = false;
+#pragma unroll
+            for (int k = SEG - 1; k >= 0; k--) {
+                m.b = advance(gate[k], m.b, delta[k]);
+                m.a *= gate[k];
+                zero |= gate[k] == 0.f;
+            }
+            m.a = keep(m.a, zero);
+        }
+        float h = in;
+        if constexpr (MAPS) {
+            box[turn][p.w][p.lane] = make_float2(m.a, m.b);
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < NW; v++) whole = compose(whole, Map{box[turn][v][p.lane].x, box[turn][v][p.lane].y});
+        } else if (NW > 1) {
+            h = join<NW>(box[turn], p.w, p.lane, m, in);
+        }
+        if (!MAPS && there) {
+#pragma unroll
+            for (int k = SEG - 1; k >= 0; k--) {
+                h = advance(gate[k], h, delta[k]);
+                if (p.on && i0 + k < a.T) {
+                    const int64_t row = (i0 + k) * n + p.c0;
+                    const bool acted = ok >> k & 1;
+                    (a.advantage + row)[p.l] = h;
+                    (a.target + row)[p.l] = acted ? h + value[k] : 0.f;
+                    (a.valid + row)[p.l] = acted;
+                }
+            }
+        }
+        if (NW == 1) in = h;
+        turn ^= 1;
+    }
+    if (MAPS && p.w == 0 && p.on) s.maps[blockIdx.y * n + p.c()] = make_float2(whole.a, whole.b);
+}
+
+// How the steps are split.  A wave keeps 2 SEG values a lane in flight; about
+// FILL waves keep the memory busy (256 CUs, 16 each).
+constexpr int64_t FILL = 4096;
+struct Split { int nw; Chunks s; };
+
+Split split_steps(int64_t T, int64_t n, float2* maps)
+{
+    const int64_t waves = (n + WAVE - 1) / WAVE, segs = (T + SEG - 1) / SEG;
+    Split r{};
+    r.nw = waves >= FILL || segs <= 1 ? 1 : waves * 4 >= FILL || segs <= 4 ? 4 : 8;
+    const int64_t tile = (int64_t)r.nw * SEG, tiles = (T + tile - 1) / tile;
+    int64_t chunks = r.nw == 8 ? FILL / (waves * r.nw) : 1;
+    chunks = chunks < 1 ? 1 : chunks > tiles ? tiles : chunks;
+    if (chunks <= 2) chunks = 1;                        // two launches do not pay for so few
+    const int64_t per = chunks > 1 ? (tiles + chunks - 1) / chunks : (tiles > 0 ? tiles : 1);
+    r.s.count = chunks > 1 ? (int32_t)((tiles + per - 1) / per) : 1;
+    r.s.steps = per * tile;
+    r.s.maps = maps;
+    return r;
 }
 
 template <class TR, class TV>
-__global__ __launch_bounds__(256) void advantages_kernel(AdvArgs a)
+void launch_advantages(const AdvArgs& a, void* workspace, hipStream_t st)
 {
-    const int64_t n = a.E * a.A, c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= n) return;
-    const int64_t e = c / a.A;
-    float carry = 0.f;
-    for (int64_t t = a.T; t-- > 0;) {
-        const int64_t i = t * n + c;
-        const uint8_t mark = a.marks[t * a.E + e];
-        const bool ok = acted(a, t, c, e, mark);
-        float target = 0.f;
-        if (ok) {
-            const bool final = a.done[i] || (mark & GW_MARK_END);
-            const float v = (float)((const TV*)a.value)[i];
-            float d = (float)((const TR*)a.reward)[i] - v;
-            if (!final) {
-                d += a.gamma * (float)((const TV*)a.value)[i + n];
-                if (!(mark & GW_MARK_TRUNCATED)) d += a.gamma * a.lam * carry;
-            }
-            carry = d;
-            target = d + v;
-        } else {
-            carry = 0.f;
-        }
-        a.advantage[i] = carry;
-        a.target[i] = target;
-        a.valid[i] = ok;
-    }
+    const int64_t n = a.E * a.A, waves = (n + WAVE - 1) / WAVE;
+    const Split q = split_steps(a.T, n, (float2*)workspace);
+    const dim3 grid((unsigned)waves, q.s.count);
+    if (q.s.count > 1) hipLaunchKernelGGL((advantages_kernel<TR, TV, 8, 1, true>), grid, dim3(512), 0, st, a, q.s);
+    if (q.nw == 1)
+        hipLaunchKernelGGL((advantages_kernel<TR, TV, 1, 4, false>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a, q.s);
+    else if (q.nw == 4) hipLaunchKernelGGL((advantages_kernel<TR, TV, 4, 1, false>), grid, dim3(256), 0, st, a, q.s);
+    else hipLaunchKernelGGL((advantages_kernel<TR, TV, 8, 1, false>), grid, dim3(512), 0, st, a, q.s);
 }
 
 template <class T, class TG>
-void launch_recurrence(const RecurArgs& a, hipStream_t st)
+void launch_recurrence(const RecurArgs& a, void* workspace, hipStream_t st)
 {
-    hipLaunchKernelGGL((recur_kernel<T, TG>), dim3((unsigned)((a.n + 255) / 256)), dim3(256), 0, st, a);
+    const Split q = split_steps(a.T, a.n, (float2*)workspace);
+    const int64_t waves = (a.n + WAVE - 1) / WAVE;
+    const dim3 grid((unsigned)waves, q.s.count);
+    if (q.s.count > 1) hipLaunchKernelGGL((maps_kernel<T, TG, 8, false>), grid, dim3(512), 0, st, a, q.s);
+    if (q.nw == 1) hipLaunchKernelGGL((recur_kernel<T, TG, 1, 4>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a, q.s);
+    else if (q.nw == 4) hipLaunchKernelGGL((recur_kernel<T, TG, 4, 1>), grid, dim3(256), 0, st, a, q.s);
+    else hipLaunchKernelGGL((recur_kernel<T, TG, 8, 1>), grid, dim3(512), 0, st, a, q.s);
+}
+
+template <class T, class TG, bool SUMS>
+void launch_backward(const RecurArgs& a, void* workspace, hipStream_t st)
+{
+    const Split q = split_steps(a.T, a.n, (float2*)workspace);
+    const int64_t waves = (a.n + WAVE - 1) / WAVE;
+    const dim3 grid((unsigned)waves, q.s.count);
+    if (q.s.count > 1) hipLaunchKernelGGL((maps_kernel<T, TG, 8, true>), grid, dim3(512), 0, st, a, q.s);
+    if (q.nw == 1)
+        hipLaunchKernelGGL((recur_backward_kernel<T, TG, 1, 4, SUMS>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a, q.s);
+    else if (q.nw == 4) hipLaunchKernelGGL((recur_backward_kernel<T, TG, 4, 1, SUMS>), grid, dim3(256), 0, st, a, q.s);
+    else hipLaunchKernelGGL((recur_backward_kernel<T, TG, 8, 1, SUMS>), grid, dim3(512), 0, st, a, q.s);
+    if (SUMS && a.parts > 1)
+        hipLaunchKernelGGL((gate_parts_kernel<TG>), dim3((unsigned)((a.T * a.gates + 255) / 256)), dim3(256), 0,
+                           st, a);
 }
 
 template <class T, class TG>
-void launch_backward(const RecurArgs& a, hipStream_t st)
+void launch_backward(const RecurArgs& a, void* workspace, hipStream_t st)
 {
-    const int64_t gates = a.n / a.gate_span;
-    const int64_t span = a.gate_span == 1 ? a.n : a.gate_span;
-    hipLaunchKernelGGL((recur_backward_kernel<T, TG>), dim3((unsigned)(a.n / span * ((span + 63) / 64))), dim3(64), 0,
-                       st, a);
-    if (a.dgate && a.gate_span > 1)
-        hipLaunchKernelGGL((gate_parts_kernel<TG>), dim3((unsigned)((a.T * gates + 255) / 256)), dim3(256), 0, st,
-                           a.part, a.parts, a.T * gates, (TG*)a.dgate);
+    if (a.dgate && a.gate_span > 1) launch_backward<T, TG, true>(a, workspace, st);
+    else launch_backward<T, TG, false>(a, workspace, st);
 }
 
 gw_status check_recurrence(int32_t dtype, int32_t gate_dtype, int64_t T, int64_t n, const void* x, const void* gate,
@@ -200,7 +572,7 @@ gw_status check_recurrence(int32_t dtype, int32_t gate_dtype, int64_t T, int64_t
     LEARN_NEED(dtype >= GW_T_F32 && dtype <= GW_T_BF16, "unknown dtype %d", dtype);
     LEARN_NEED(gate_dtype == dtype || gate_dtype == GW_T_F32, "gate_dtype %d with dtype %d: the same or GW_T_F32",
                gate_dtype, dtype);
-    LEARN_NEED(T >= 0 && n >= 0 && T <= (INT64_C(1) << 31) && n <= (INT64_C(1) << 31), "%lld steps of %lld channels",
+    LEARN_NEED(T >= 0 && n >= 0 && T <= (INT64_C(1) << 31) && n < (INT64_C(1) << 31), "%lld steps of %lld channels",
                (long long)T, (long long)n);
     LEARN_NEED(T == 0 || n == 0 || x, "x: null pointer");
     LEARN_NEED(gate_span >= 1 && n % gate_span == 0, "gate_span %lld for %lld channels", (long long)gate_span, (long long)n);
@@ -210,17 +582,20 @@ gw_status check_recurrence(int32_t dtype, int32_t gate_dtype, int64_t T, int64_t
     return GW_OK;
 }
 
-int64_t gate_pieces(int64_t gate_span) { return (gate_span + 63) / 64; }
+// parts of a shared gate's sum: the waves that its channels can lie in
+int64_t gate_pieces(int64_t gate_span) { return WAVE % gate_span == 0 ? 1 : (gate_span - 1) / WAVE + 2; }
+
+int64_t maps_bytes(int64_t T, int64_t n)
+{
+    const Split q = split_steps(T, n, nullptr);
+    return q.s.count > 1 ? q.s.count * n * (int64_t)sizeof(float2) : 0;
+}
 
 }  // namespace
 
 extern "C" {
 
-int64_t gw_recurrence_workspace(int64_t n_steps, int64_t n)
-{
-    (void)n_steps; (void)n;
-    return 0;
-}
+int64_t gw_recurrence_workspace(int64_t n_steps, int64_t n) { return n_steps <= 0 || n <= 0 ? 0 : maps_bytes(n_steps, n); }
 
 gw_status gw_recurrence(int32_t dtype, int32_t gate_dtype, int64_t n_steps, int64_t n,
                         const void* x, const void* gate, int64_t gate_span, float gate_value,
@@ -228,27 +603,31 @@ gw_status gw_recurrence(int32_t dtype, int32_t gate_dtype, int64_t n_steps, int6
                         void* h, float* last, float* carry,
                         void* workspace, int64_t workspace_bytes, void* stream)
 {
-    (void)workspace; (void)workspace_bytes;
     const gw_status s = check_recurrence(dtype, gate_dtype, n_steps, n, x, gate, gate_span, gate_value, cut, cut_span);
     if (s != GW_OK) return s;
     LEARN_NEED(n_steps == 0 || n == 0 || h, "h: null pointer");
+    const int64_t need = gw_recurrence_workspace(n_steps, n);
+    LEARN_NEED(need == 0 || (workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= need),
+               "workspace: %lld bytes, 8-byte aligned, are needed", (long long)need);
     if (n == 0) return GW_OK;
     RecurArgs a{};
-    a.T = n_steps; a.n = n; a.x = x; a.gate = gate; a.gate_span = gate_span; a.gate_value = gate_value;
-    a.cut = cut; a.cut_span = cut_span; a.state = state; a.reverse = reverse;
+    a.T = n_steps; a.n = n; a.x = x; a.gate = gate; a.gate_span = (uint32_t)gate_span; a.gate_value = gate_value;
+    a.cut = cut; a.cut_span = cut ? (uint32_t)cut_span : 1; a.gates = n / gate_span; a.cuts = n / a.cut_span;
+    a.state = state; a.reverse = reverse;
     a.h = h; a.last = last; a.carry = carry;
     const hipStream_t st = (hipStream_t)stream;
-    if (dtype == GW_T_F32) launch_recurrence<float, float>(a, st);
-    else if (dtype == GW_T_F16) gate_dtype == dtype ? launch_recurrence<f16, f16>(a, st) : launch_recurrence<f16, float>(a, st);
-    else gate_dtype == dtype ? launch_recurrence<bf16, bf16>(a, st) : launch_recurrence<bf16, float>(a, st);
+    if (dtype == GW_T_F32) launch_recurrence<float, float>(a, workspace, st);
+    else if (dtype == GW_T_F16) gate_dtype == dtype ? launch_recurrence<f16, f16>(a, workspace, st) : launch_recurrence<f16, float>(a, workspace, st);
+    else gate_dtype == dtype ? launch_recurrence<bf16, bf16>(a, workspace, st) : launch_recurrence<bf16, float>(a, workspace, st);
     LEARN_LAUNCHED();
     return GW_OK;
 }
 
 int64_t gw_recurrence_backward_workspace(int64_t n_steps, int64_t n, int64_t gate_span)
 {
-    if (n_steps <= 0 || n <= 0 || gate_span <= 1) return 0;
-    return n_steps * (n / gate_span) * gate_pieces(gate_span) * 4;
+    if (n_steps <= 0 || n <= 0 || gate_span < 1) return 0;
+    const int64_t pieces = gate_span > 1 ? gate_pieces(gate_span) : 1;
+    return maps_bytes(n_steps, n) + (pieces > 1 ? n_steps * (n / gate_span) * pieces * 4 : 0);
 }
 
 gw_status gw_recurrence_backward(int32_t dtype, int32_t gate_dtype, int64_t n_steps, int64_t n,
@@ -262,19 +641,20 @@ gw_status gw_recurrence_backward(int32_t dtype, int32_t gate_dtype, int64_t n_st
     if (s != GW_OK) return s;
     LEARN_NEED(n_steps == 0 || n == 0 || (carry && dx), "carry or dx: null pointer");
     LEARN_NEED(!dgate || gate, "dgate without gate");
-    const int64_t need = dgate ? gw_recurrence_backward_workspace(n_steps, n, gate_span) : 0;
+    const int64_t need = gw_recurrence_backward_workspace(n_steps, n, gate_span);
     LEARN_NEED(need == 0 || (workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= need),
                "workspace: %lld bytes, 8-byte aligned, are needed", (long long)need);
     if (n == 0) return GW_OK;
     RecurArgs a{};
-    a.T = n_steps; a.n = n; a.x = x; a.gate = gate; a.gate_span = gate_span; a.gate_value = gate_value;
-    a.cut = cut; a.cut_span = cut_span; a.reverse = reverse; a.carry = const_cast<float*>(carry);
+    a.T = n_steps; a.n = n; a.x = x; a.gate = gate; a.gate_span = (uint32_t)gate_span; a.gate_value = gate_value;
+    a.cut = cut; a.cut_span = cut ? (uint32_t)cut_span : 1; a.gates = n / gate_span; a.cuts = n / a.cut_span;
+    a.reverse = reverse; a.carry = const_cast<float*>(carry);
     a.dh = dh; a.dlast = dlast; a.dx = dx; a.dgate = dgate; a.dstate = dstate;
-    a.part = (float*)workspace; a.parts = (int32_t)gate_pieces(gate_span);
+    a.part = (float*)((char*)workspace + maps_bytes(n_steps, n)); a.parts = (int32_t)gate_pieces(gate_span);
     const hipStream_t st = (hipStream_t)stream;
-    if (dtype == GW_T_F32) launch_backward<float, float>(a, st);
-    else if (dtype == GW_T_F16) gate_dtype == dtype ? launch_backward<f16, f16>(a, st) : launch_backward<f16, float>(a, st);
-    else gate_dtype == dtype ? launch_backward<bf16, bf16>(a, st) : launch_backward<bf16, float>(a, st);
+    if (dtype == GW_T_F32) launch_backward<float, float>(a, workspace, st);
+    else if (dtype == GW_T_F16) gate_dtype == dtype ? launch_backward<f16, f16>(a, workspace, st) : launch_backward<f16, float>(a, workspace, st);
+    else gate_dtype == dtype ? launch_backward<bf16, bf16>(a, workspace, st) : launch_backward<bf16, float>(a, workspace, st);
     LEARN_LAUNCHED();
     return GW_OK;
 }
@@ -300,27 +680,27 @@ gw_status gw_advantages(int32_t dtype, int32_t reward_f64, int64_t n_steps, int6
                         float* advantage, float* target, uint8_t* valid,
                         void* workspace, int64_t workspace_bytes, void* stream)
 {
-    (void)workspace; (void)workspace_bytes;
     LEARN_NEED(dtype >= GW_T_F32 && dtype <= GW_T_BF16, "unknown dtype %d", dtype);
-    LEARN_NEED(n_steps >= 0 && n_envs >= 0 && n_lanes >= 1 && n_envs <= (INT64_C(1) << 31) / n_lanes,
+    LEARN_NEED(n_steps >= 0 && n_envs >= 0 && n_lanes >= 1 && n_lanes < (INT64_C(1) << 31) &&
+                   n_envs <= ((INT64_C(1) << 31) - 1) / n_lanes,
                "%lld steps of %lld envs of %lld lanes", (long long)n_steps, (long long)n_envs, (long long)n_lanes);
     LEARN_NEED(isfinite(gamma) && isfinite(lam), "gamma or lam is not finite");
     if (n_steps == 0 || n_envs == 0) return GW_OK;
     LEARN_NEED(reward && value && done && marks && live && advantage && target && valid, "null pointer");
     const AdvArgs a{n_steps, n_envs, n_lanes, reward, value, done, marks, live, acts, gamma, lam, advantage, target, valid};
-    const dim3 grid((unsigned)((n_envs * n_lanes + 255) / 256));
+    const int64_t need = gw_recurrence_workspace(n_steps, n_envs * n_lanes);
+    LEARN_NEED(need == 0 || (workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= need),
+               "workspace: %lld bytes, 8-byte aligned, are needed", (long long)need);
     const hipStream_t st = (hipStream_t)stream;
-#define ADV(TR, TV) hipLaunchKernelGGL((advantages_kernel<TR, TV>), grid, dim3(256), 0, st, a)
     if (reward_f64) {
-        if (dtype == GW_T_F32) ADV(double, float);
-        else if (dtype == GW_T_F16) ADV(double, f16);
-        else ADV(double, bf16);
+        if (dtype == GW_T_F32) launch_advantages<double, float>(a, workspace, st);
+        else if (dtype == GW_T_F16) launch_advantages<double, f16>(a, workspace, st);
+        else launch_advantages<double, bf16>(a, workspace, st);
     } else {
-        if (dtype == GW_T_F32) ADV(float, float);
-        else if (dtype == GW_T_F16) ADV(float, f16);
-        else ADV(float, bf16);
+        if (dtype == GW_T_F32) launch_advantages<float, float>(a, workspace, st);
+        else if (dtype == GW_T_F16) launch_advantages<float, f16>(a, workspace, st);
+        else launch_advantages<float, bf16>(a, workspace, st);
     }
-#undef ADV
     LEARN_LAUNCHED();
     return GW_OK;
 }

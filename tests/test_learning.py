@@ -171,7 +171,7 @@ def test_c_entries_refuse_without_a_gpu():
                        (12, None, 'h')]:
         bad.append((L.gw_recurrence, rec[:i] + [v] + rec[i + 1:], word))
     bad.append((L.gw_recurrence, rec[:8] + [one, 3] + rec[10:], 'cut_span'))
-    back = [0, 0, 3, 4, one, one, 2, 0.0, None, 1, one, 0, None, None, one, one, None, None, 0, None]
+    back = [0, 0, 3, 6, one, one, 3, 0.0, None, 1, one, 0, None, None, one, one, None, None, 0, None]
     bad.append((L.gw_recurrence_backward, back, 'workspace'))
     bad.append((L.gw_recurrence_backward, back[:5] + [None] + back[6:], 'dgate'))
     bad.append((L.gw_recurrence_backward, back[:10] + [None] + back[11:], 'carry'))
