@@ -104,7 +104,8 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
             for (int d = 0; d < h.n; d++) owned |= h.slot[d] == c;
             if (!owned) act[c] = 0;
         }
-        float logp = 0.f, entropy = 0.f;
+        double logp = 0.;
+        float entropy = 0.f;
         for (int d = 0; d < h.n; d++) {
             const int lo = h.off[d], hi = h.off[d + 1];
             float m = NEG_INF, bs = NEG_INF;
@@ -146,12 +147,12 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
             s = grp.sum(s);
             t = grp.sum(t);
             const float log_s = logf(s);
-            logp += (logit_at(z, mask, bi) - m) - log_s;
+            logp += (double)(logit_at(z, mask, bi) - m) - (double)log_s;
             entropy += log_s - t / s;
             if (tid == 0) act[h.slot[d]] = h.low[d] + (bi - lo);
         }
         if (tid == 0) {
-            if (a.logp) a.logp[row] = logp;
+            if (a.logp) a.logp[row] = (float)logp;
             if (a.entropy) a.entropy[row] = entropy;
         }
     }
@@ -163,12 +164,14 @@ struct RowLoss {
     bool clipped;
 };
 
-__device__ inline RowLoss row_loss(const LossArgs& a, int64_t row, float logp, bool possible, float kl, float entropy)
+// (L is a sum of numbers near its own size: in double its difference to
+// old_logp, which is near 0, is exact to the heads' own errors)
+__device__ inline RowLoss row_loss(const LossArgs& a, int64_t row, double logp, bool possible, float kl, float entropy)
 {
     RowLoss r;
-    r.logp = possible ? logp : NEG_INF;
+    r.logp = possible ? (float)logp : NEG_INF;
     const float adv = a.advantage[row];
-    const float ratio = possible ? expf(logp - a.old_logp[row]) : 0.f;
+    const float ratio = possible ? expf((float)(logp - (double)a.old_logp[row])) : 0.f;
     const float clamped = fminf(fmaxf(ratio, a.lo), a.hi);
     const float free = ratio * adv, held = (ratio != ratio ? ratio : clamped) * adv;
     r.clipped = held < free;
@@ -186,9 +189,10 @@ __device__ inline float inverse_rows(const LossArgs& a)
     float m;
     if (a.denominator_at) m = *a.denominator_at;
     else if (a.counts) {
+        // (every wave adds the blocks' counts: fewer than 2^31 rows a block)
         int64_t n = 0;
-        for (int i = 0; i < a.n_counts; i++) n += a.counts[i];
-        m = (float)n;
+        for (int i = threadIdx.x & 63; i < a.n_counts; i += WAVE) n += a.counts[i];
+        m = (float)wave_sum(n);
     } else m = (float)a.rows;
     return m > 0.f ? 1.f / m : 0.f;
 }
@@ -205,6 +209,332 @@ __device__ inline void write_out(const LossArgs& a, const double* s)
     a.out[3] = (float)(s[S_H] * inv);
     a.out[4] = (float)(s[S_CLIP] * inv);
     a.out[5] = (float)m;
+}
+
+// ------------------------------------------------------------ rows out of registers
+template <class T, int CM>
+__device__ inline void store_row(T* row, int width, const float* v)
+{
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+    for (int u = 0; u < CM / PER; u++) {
+        if (u * PER >= width) continue;
+        T t[PER];
+#pragma unroll
+        for (int e = 0; e < PER; e++) t[e] = (T)v[u * PER + e];
+        uint4 w;
+        __builtin_memcpy(&w, t, 16);
+        ((uint4*)row)[u] = w;
+    }
+}
+
+// a lane's row into the wave's tile in LDS (rows side by side)
+template <class T, int CM>
+__device__ inline void write_tile(T* row, int width, const float* v)
+{
+    if (sizeof(T) == 2 && (width & 1) == 0) {
+#pragma unroll
+        for (int j = 0; j < CM; j += 2) {
+            if (j >= width) continue;
+            const T t[2] = {(T)v[j], (T)v[j + 1]};
+            uint32_t w;
+            __builtin_memcpy(&w, t, sizeof(T) == 2 ? 4 : 0);
+            ((uint32_t*)row)[j / 2] = w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < CM; j++)
+            if (j < width) row[j] = (T)v[j];
+    }
+}
+
+// the tile to memory, side by side there too
+template <class T>
+__device__ inline void copy_tile(const T* tile, T* to, int n, bool wide, int lane)
+{
+    constexpr int PER = 16 / sizeof(T);
+    int done = 0;
+    if (wide) {
+        done = n / PER * PER;
+        for (int i = lane; i < n / PER; i += WAVE) ((uint4*)to)[i] = ((const uint4*)tile)[i];
+    }
+    for (int i = done + lane; i < n; i += WAVE) to[i] = tile[i];
+}
+
+// a workgroup's sums: to its place among the partial ones, or, where it is the only one, to out
+template <int WAVES>
+__device__ inline void block_sums(const LossArgs& a, double* s)
+{
+    __shared__ double box[WAVES][N_SUMS];
+#pragma unroll
+    for (int k = 0; k < N_SUMS; k++) s[k] = wave_sum(s[k]);
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0)
+            for (int k = 0; k < N_SUMS; k++) box[threadIdx.x >> 6][k] = s[k];
+        __syncthreads();
+        if (threadIdx.x != 0) return;
+        for (int w = 1; w < WAVES; w++)
+            for (int k = 0; k < N_SUMS; k++) s[k] += box[w][k];
+    }
+    if (threadIdx.x != 0) return;
+    if (gridDim.x == 1) write_out(a, s);
+    else
+        for (int k = 0; k < N_SUMS; k++) a.partial[(int64_t)k * gridDim.x + blockIdx.x] = s[k];
+}
+
+// ------------------------------------------------------------- narrow rows
+// A thread a row, the whole row in registers (CM: the width, rounded up).
+// Where the heads begin and end is uniform, so the sweeps over a row are
+// unrolled and a head's end is a scalar branch: no lane of a wave idles, no
+// reduction crosses lanes, and the memory sees each value once.  A choice that
+// does not exist holds NO_CHOICE, whose exponential is 0.
+constexpr int NARROW = 48;
+constexpr float NO_CHOICE = -1e30f;
+
+struct Small {
+    int32_t n, act_dim, width, owned;           // owned: every action column has a head
+    uint64_t starts, ends;                      // bit j: choice j is a head's first, last
+    int32_t low[NARROW];
+    int16_t slot[NARROW];
+    int32_t unit, unit_ref, unit_mask, unit_grad, unit_noise;  // bytes that a row's loads and stores may take at once
+};
+
+template <class T, int CM, class W>
+__device__ inline void load_units(const T* row, int width, float* v)
+{
+    constexpr int PER = sizeof(W) / sizeof(T);
+    W w[CM / PER];
+#pragma unroll
+    for (int u = 0; u < CM / PER; u++)
+        if (u * PER < width) w[u] = ((const W*)row)[u];
+#pragma unroll
+    for (int u = 0; u < CM / PER; u++) {
+        T t[PER];
+        __builtin_memcpy(t, &w[u], sizeof(W));
+#pragma unroll
+        for (int e = 0; e < PER; e++) v[u * PER + e] = u * PER + e < width ? (float)t[e] : NEG_INF;
+    }
+}
+
+// a row of `width` <= CM values, -inf behind them
+template <class T, int CM>
+__device__ inline void load_row(const T* row, int width, int unit, float* v)
+{
+    if constexpr (CM * sizeof(T) % 16 == 0) {
+        if (unit == 16) return load_units<T, CM, uint4>(row, width, v);
+    }
+    if (unit >= 8) load_units<T, CM, uint2>(row, width, v);
+    else if (unit >= 4) load_units<T, CM, uint32_t>(row, width, v);
+    else load_units<T, CM, T>(row, width, v);
+}
+
+// e^x: for 16-bit logits the hardware's 2^x, 2^-20 near for |x| < 16 and far
+// below their own step; for float32 the library's
+template <class T>
+__device__ inline float exp_of(float x)
+{
+    if constexpr (sizeof(T) == 4) return expf(x);
+    return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
+}
+
+__device__ inline bool bit(uint64_t b, int j) { return b >> j & 1; }
+
+// v[j] less its head's maximum (0 where a head has no choice; NaN stays)
+template <int CM>
+__device__ inline void subtract_max(const Small& h, float* v)
+{
+    float m[CM];
+#pragma unroll
+    for (int j = 0; j < CM; j++) m[j] = j == 0 ? v[0] : fmaxf(v[j], bit(h.starts, j) ? NEG_INF : m[j - 1]);
+    float top = 0.f;
+#pragma unroll
+    for (int j = CM - 1; j >= 0; j--) {
+        if (bit(h.ends, j)) top = m[j] == NEG_INF ? 0.f : m[j];
+        v[j] = v[j] == NEG_INF ? NO_CHOICE : v[j] - top;
+    }
+}
+
+// masked choices of the row to -inf; row r uses mask row r % mask_rows
+template <int CM>
+__device__ inline void apply_mask(const uint8_t* mask, int64_t mask_rows, int64_t tile_row, int lane, int width, int unit,
+                                  float* v)
+{
+    int64_t r = tile_row % mask_rows + lane;
+    r = mask_rows >= WAVE ? (r >= mask_rows ? r - mask_rows : r) : (int64_t)((uint32_t)r % (uint32_t)mask_rows);
+    float m[CM];
+    load_row<uint8_t, CM>(mask + r * width, width, unit, m);
+#pragma unroll
+    for (int j = 0; j < CM; j++) v[j] = m[j] == 0.f ? NEG_INF : v[j];
+}
+
+template <class T, int CM>
+__global__ __launch_bounds__(256) void sample_narrow_kernel(SampleArgs a, Small h)
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t tiles = (a.rows + WAVE - 1) / WAVE, waves = (int64_t)gridDim.x * 4;
+    for (int64_t tile = (int64_t)blockIdx.x * 4 + wave; tile < tiles; tile += waves) {
+        const int64_t base = tile * WAVE, row = base + lane < a.rows ? base + lane : a.rows - 1;
+        const bool there = base + lane < a.rows;
+        float v[CM], s[CM];
+        load_row<T, CM>((const T*)a.logits + row * a.ld, h.width, h.unit, v);
+        if (a.noise) load_row<float, CM>(a.noise + row * h.width, h.width, h.unit_noise, s);
+        if (a.mask) apply_mask<CM>(a.mask, a.mask_rows, base, (int)(row - base), h.width, h.unit_mask, v);
+#pragma unroll
+        for (int j = 0; j < CM; j++) s[j] = a.noise ? v[j] + s[j] : v[j];
+        float raw[CM];
+#pragma unroll
+        for (int j = 0; j < CM; j++) raw[j] = v[j];
+        subtract_max<CM>(h, v);
+        float sum = 0.f, t = 0.f, best = NEG_INF, at = __builtin_nanf("");
+        int choice = -1, d = 0, first = 0;
+        double logp = 0.;
+        float entropy = 0.f;
+        int32_t* act = a.actions + row * h.act_dim;
+#pragma unroll
+        for (int j = 0; j < CM; j++) {
+            const float e = exp_of<T>(v[j]);
+            sum += e;
+            t += e * v[j];
+            // the first of the largest scores; a score of -inf counts for a choice that exists
+            const bool better = raw[j] != NEG_INF && (s[j] > best || (choice < 0 && s[j] == best));
+            best = better ? s[j] : best;
+            choice = better ? j : choice;
+            at = better ? v[j] : at;
+            if (bit(h.ends, j)) {
+                const bool some = sum != 0.f;
+                const float log_s = some ? logf(sum) : 0.f;
+                logp += some ? (double)at - (double)log_s : 0.;
+                entropy += some ? log_s - t / sum : 0.f;
+                if (there) act[h.slot[d]] = h.low[d] + (choice < 0 ? 0 : choice - first);
+                sum = t = 0.f;
+                best = NEG_INF;
+                at = __builtin_nanf("");
+                choice = -1;
+                first = j + 1;
+                d++;
+            }
+        }
+        if (!there) continue;
+        if (!h.owned)
+            for (int c = 0; c < h.act_dim; c++) {
+                bool has = false;
+                for (int k = 0; k < h.n; k++) has |= h.slot[k] == c;
+                if (!has) act[c] = 0;
+            }
+        if (a.logp) a.logp[row] = (float)logp;
+        if (a.entropy) a.entropy[row] = entropy;
+    }
+}
+
+// What the gradient needs of a head again: 1/S, T/S, 1/S of ref, the choice's place
+typedef float4 HeadBox;
+
+template <class T, int CM, bool REF, bool GRAD>
+__global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
+{
+    extern __shared__ float4 lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    // per wave: [heads][64] boxes, then the tile of gradients
+    const int tile_bytes = GRAD && h.unit_grad < 0 ? (WAVE * h.width * (int)sizeof(T) + 15) & ~15 : 0;
+    char* mine = (char*)lds + wave * ((GRAD ? h.n * WAVE * (int)sizeof(HeadBox) : 0) + tile_bytes);
+    HeadBox* boxes = (HeadBox*)mine;
+    T* out = (T*)(mine + h.n * WAVE * sizeof(HeadBox));
+    const int64_t tiles = (a.rows + WAVE - 1) / WAVE, waves = (int64_t)gridDim.x * 4;
+    float step = 0.f;
+    if (GRAD) step = a.scale * (a.upstream ? *a.upstream : 1.f) * inverse_rows(a);
+    double sums[N_SUMS] = {0., 0., 0., 0., 0.};
+    for (int64_t tile = (int64_t)blockIdx.x * 4 + wave; tile < tiles; tile += waves) {
+        const int64_t base = tile * WAVE, row = base + lane < a.rows ? base + lane : a.rows - 1;
+        const bool there = base + lane < a.rows, valid = there && (!a.valid || a.valid[row]);
+        float x[CM], y[REF ? CM : 1], e[CM];
+        load_row<T, CM>((const T*)a.logits + row * a.ld, h.width, h.unit, x);
+        if constexpr (REF) load_row<T, CM>((const T*)a.ref + row * a.ld_ref, h.width, h.unit_ref, y);
+        if (a.mask) apply_mask<CM>(a.mask, a.mask_rows, base, (int)(row - base), h.width, h.unit_mask, x);
+        if constexpr (REF) {
+#pragma unroll
+            for (int j = 0; j < CM; j++) y[j] = x[j] == NEG_INF ? NEG_INF : y[j];
+            subtract_max<CM>(h, y);
+        }
+        subtract_max<CM>(h, x);
+        const int32_t* act = a.actions + row * h.act_dim;
+        float s = 0.f, t = 0.f, sr = 0.f, u = 0.f, at = 0.f, kl = 0.f, entropy = 0.f;
+        double logp = 0.;
+        bool possible = true, found = false;
+        int d = 0, first = 0;
+        uint32_t chosen = (uint32_t)act[h.slot[0]] - (uint32_t)h.low[0];
+#pragma unroll
+        for (int j = 0; j < CM; j++) {
+            e[j] = exp_of<T>(x[j]);
+            s += e[j];
+            t += e[j] * x[j];
+            const bool it = (uint32_t)(j - first) == chosen && x[j] != NO_CHOICE;
+            at = it ? x[j] : at;
+            found |= it;
+            if constexpr (REF) {
+                const float er = exp_of<T>(y[j]);
+                sr += er;
+                u += er * (y[j] - x[j]);
+                y[j] = er;
+            }
+            if (bit(h.ends, j)) {
+                const bool some = s != 0.f, some_ref = REF && some && sr != 0.f;
+                const float inv = some ? 1.f / s : 0.f, log_s = some ? logf(s) : 0.f, ts = t * inv;
+                const float inv_r = some_ref ? 1.f / sr : 0.f;
+                entropy += log_s - ts;
+                if (some_ref) kl += u * inv_r + (log_s - logf(sr));
+                possible &= found || !some;
+                logp += found ? (double)at - (double)log_s : 0.;
+                if (GRAD) boxes[d * WAVE + lane] = make_float4(inv, ts, inv_r, __int_as_float(found ? first + (int)chosen : -1));
+                s = t = sr = u = 0.f;
+                found = false;
+                first = j + 1;
+                d++;
+                if (d < h.n) chosen = (uint32_t)act[h.slot[d]] - (uint32_t)h.low[d];
+            }
+        }
+        const RowLoss r = row_loss(a, row, logp, possible, kl, entropy);
+        if (a.logp && there) a.logp[row] = valid ? r.logp : 0.f;
+        if (valid) {
+            sums[S_PG] += r.pg; sums[S_KL] += r.kl; sums[S_H] += r.entropy;
+            sums[S_CLIP] += r.clipped ? 1. : 0.; sums[S_COUNT] += 1.;
+        }
+        if constexpr (GRAD) {
+            const float pull = r.pull * step, eta = a.entropy * step, beta = a.kl * step;
+            float a0 = 0.f, a1 = 0.f, b = 0.f;
+            int place = -1;
+            wave_sync();
+#pragma unroll
+            for (int j = CM - 1; j >= 0; j--) {
+                if (bit(h.ends, j)) {
+                    d--;
+                    const HeadBox q = boxes[d * WAVE + lane];
+                    // g = e/S ((beta - pull) + eta (x - T/S)) - beta er/Sr, and pull at the choice:
+                    // log p + H = x - T/S
+                    a1 = eta * q.x;
+                    a0 = q.x * ((q.z != 0.f ? beta : 0.f) - pull - eta * q.y);
+                    b = -beta * q.z;
+                    place = __float_as_int(q.w);
+                }
+                float g = e[j] * fmaf(a1, x[j], a0);
+                if constexpr (REF) g = fmaf(b, y[j], g);
+                g += place == j ? pull : 0.f;
+                x[j] = valid && x[j] != NO_CHOICE ? g : 0.f;
+            }
+            T* grad = (T*)a.grad + base * h.width;
+            if (h.unit_grad > 0) {
+                // rows of one or two 16-byte pieces: straight from the registers
+                if (there) store_row<T, CM>(grad + lane * h.width, h.width, x);
+            } else {
+                write_tile<T, CM>(out + lane * h.width, h.width, x);
+                wave_sync();
+                const int64_t rows = a.rows - base < WAVE ? a.rows - base : WAVE;
+                copy_tile<T>(out, grad, (int)rows * h.width, h.unit_grad == -16, lane);
+                wave_sync();
+            }
+        }
+    }
+    if (!a.out) return;
+    block_sums<4>(a, sums);
 }
 
 // One row by one workgroup of G threads, as sample_rows_kernel: maximum,
@@ -232,7 +562,8 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
         const T* zr = a.ref ? (const T*)a.ref + row * a.ld_ref : nullptr;
         const uint8_t* mask = a.mask ? a.mask + (row % a.mask_rows) * h.width : nullptr;
         const int32_t* act = a.actions + row * h.act_dim;
-        float logp = 0.f, kl = 0.f, entropy = 0.f;
+        float kl = 0.f, entropy = 0.f;
+        double logp = 0.;
         bool possible = true;
         for (int d = 0; d < h.n; d++) {
             const int lo = h.off[d], hi = h.off[d + 1];
@@ -275,7 +606,7 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                 const int c = act[h.slot[d]] - h.low[d];
                 const float v = c >= 0 && c < hi - lo ? logit_at(z, mask, lo + c) : NEG_INF;
                 if (v == NEG_INF) possible = false;
-                else logp += (v - m) - log_s;
+                else logp += (double)(v - m) - (double)log_s;
             }
             if (tid == 0) {
                 hm[d] = m; hls[d] = log_s; hinv[d] = inv; hh[d] = ent; hrm[d] = mr; hrinv[d] = inv_r;
@@ -305,22 +636,30 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
         }
         __syncthreads();
     }
-    if (!a.out || tid != 0) return;
-    if (gridDim.x == 1) write_out(a, sums);
-    else
-        for (int k = 0; k < N_SUMS; k++) a.partial[(int64_t)blockIdx.x * N_SUMS + k] = sums[k];
+    if (!a.out || tid >= WAVE) return;
+    block_sums<1>(a, sums);
 }
 
 constexpr int COUNT_BLOCKS = 256;
 
-// valid rows, counted per block
-__global__ __launch_bounds__(256) void count_kernel(const uint8_t* valid, int64_t rows, int32_t* counts)
+// valid rows, counted per block; `wide`: the flags are 16-byte aligned
+__global__ __launch_bounds__(256) void count_kernel(const uint8_t* valid, int64_t rows, int wide, int32_t* counts)
 {
     __shared__ int box[4];
-    const int64_t per = (rows + gridDim.x - 1) / gridDim.x, from = per * blockIdx.x;
-    const int64_t to = from + per < rows ? from + per : rows;
+    const int64_t pieces = wide ? rows / 16 : 0;
     int n = 0;
-    for (int64_t i = from + threadIdx.x; i < to; i += 256) n += valid[i] != 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
+        const uint4 v = ((const uint4*)valid)[i];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            // 0x80 in each byte that is not 0
+            const uint32_t t = ((w[k] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[k];
+            n += __popc(t & 0x80808080u);
+        }
+    }
+    for (int64_t i = pieces * 16 + (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows; i += (int64_t)gridDim.x * 256)
+        n += valid[i] != 0;
     n = wave_sum(n);
     if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = n;
     __syncthreads();
@@ -328,20 +667,21 @@ __global__ __launch_bounds__(256) void count_kernel(const uint8_t* valid, int64_
 }
 
 // the blocks' partial sums, added in a fixed order, to the loss and its parts
-__global__ __launch_bounds__(256) void finish_kernel(LossArgs a, int blocks)
+__global__ __launch_bounds__(512) void finish_kernel(LossArgs a, int blocks)
 {
-    __shared__ double box[4][N_SUMS];
-    double s[N_SUMS] = {0., 0., 0., 0., 0.};
-    for (int b = threadIdx.x; b < blocks; b += 256)
-        for (int k = 0; k < N_SUMS; k++) s[k] += a.partial[(int64_t)b * N_SUMS + k];
-    for (int k = 0; k < N_SUMS; k++) s[k] = wave_sum(s[k]);
-    if ((threadIdx.x & 63) == 0)
-        for (int k = 0; k < N_SUMS; k++) box[threadIdx.x >> 6][k] = s[k];
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    for (int w = 1; w < 4; w++)
-        for (int k = 0; k < N_SUMS; k++) s[k] += box[w][k];
-    write_out(a, s);
+    __shared__ double box[8];
+    __shared__ double total[N_SUMS];
+    for (int k = 0; k < N_SUMS; k++) {
+        double s = 0.;
+        for (int b = threadIdx.x; b < blocks; b += 512) s += a.partial[(int64_t)k * blocks + b];
+        s = wave_sum(s);
+        if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = s;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            total[k] = ((box[0] + box[1]) + (box[2] + box[3])) + ((box[4] + box[5]) + (box[6] + box[7]));
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) write_out(a, total);
 }
 
 constexpr int MAX_BLOCKS = 8192;
@@ -373,19 +713,108 @@ gw_status take_heads(const gw_policy_heads* p, Heads* h)
 
 int64_t blocks_for(int64_t rows) { return rows < MAX_BLOCKS ? rows : MAX_BLOCKS; }
 
+// the largest piece (a power of two up to 16 bytes) in which rows of this many
+// bytes, that far apart, can be read from there
+int unit_of(const void* p, int64_t row_bytes, int64_t apart, int64_t rows)
+{
+    uintptr_t u = (uintptr_t)p | (uintptr_t)row_bytes | (rows > 1 ? (uintptr_t)apart : 0) | 16;
+    return (int)(u & -u);
+}
+
+// the narrow kernels' heads, or false if the rows are not narrow
+bool take_small(const Heads& h, Small* s)
+{
+    if (h.width > NARROW) return false;
+    *s = Small{};
+    s->n = h.n; s->act_dim = h.act_dim; s->width = h.width; s->owned = h.n == h.act_dim;
+    for (int d = 0; d < h.n; d++) {
+        s->starts |= UINT64_C(1) << h.off[d];
+        s->ends |= UINT64_C(1) << (h.off[d + 1] - 1);
+        s->low[d] = h.low[d];
+        s->slot[d] = h.slot[d];
+    }
+    return true;
+}
+
+constexpr int64_t NARROW_BLOCKS = 2048;         // 256 CUs, 8 workgroups of 4 waves each
+
+unsigned narrow_blocks(int64_t rows)
+{
+    const int64_t tiles = (rows + 4 * WAVE - 1) / (4 * WAVE);
+    return (unsigned)(tiles < NARROW_BLOCKS ? tiles : NARROW_BLOCKS);
+}
+
+template <class T, int CM>
+void launch_sample_narrow(const SampleArgs& a, const Small& s, hipStream_t st)
+{
+    hipLaunchKernelGGL((sample_narrow_kernel<T, CM>), dim3(narrow_blocks(a.rows)), dim3(256), 0, st, a, s);
+}
+
 template <class T>
 void launch_sample(const SampleArgs& a, const Heads& h, hipStream_t st)
 {
+    Small s;
+    if (take_small(h, &s)) {
+        s.unit = unit_of(a.logits, h.width * sizeof(T), a.ld * sizeof(T), a.rows);
+        s.unit_noise = unit_of(a.noise, h.width * 4, h.width * 4, a.rows);
+        s.unit_mask = unit_of(a.mask, h.width, h.width, a.rows);
+        if (h.width <= 8) launch_sample_narrow<T, 8>(a, s, st);
+        else if (h.width <= 16) launch_sample_narrow<T, 16>(a, s, st);
+        else if (h.width <= 32) launch_sample_narrow<T, 32>(a, s, st);
+        else launch_sample_narrow<T, 48>(a, s, st);
+        return;
+    }
     const dim3 grid((unsigned)blocks_for(a.rows));
     if (h.width >= 1024) hipLaunchKernelGGL((sample_rows_kernel<T, 256>), grid, dim3(256), 0, st, a, h);
     else hipLaunchKernelGGL((sample_rows_kernel<T, 64>), grid, dim3(64), 0, st, a, h);
 }
 
-template <class T>
-void launch_loss(const LossArgs& a, const Heads& h, unsigned blocks, hipStream_t st)
+template <class T, int CM, bool REF>
+void launch_loss_narrow(const LossArgs& a, const Small& s, unsigned blocks, hipStream_t st)
 {
+    size_t lds = 0;
+    if (a.grad) {
+        lds = 4 * ((size_t)s.n * WAVE * sizeof(HeadBox) + (s.unit_grad < 0 ? (WAVE * s.width * sizeof(T) + 15) & ~(size_t)15 : 0));
+        const void* k = (const void*)loss_narrow_kernel<T, CM, REF, true>;
+        if (lds > 64 * 1024) (void)hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        hipLaunchKernelGGL((loss_narrow_kernel<T, CM, REF, true>), dim3(blocks), dim3(256), lds, st, a, s);
+    } else {
+        hipLaunchKernelGGL((loss_narrow_kernel<T, CM, REF, false>), dim3(blocks), dim3(256), lds, st, a, s);
+    }
+}
+
+template <class T, int CM>
+void launch_loss_narrow(const LossArgs& a, const Small& s, unsigned blocks, hipStream_t st)
+{
+    if (a.ref) launch_loss_narrow<T, CM, true>(a, s, blocks, st);
+    else launch_loss_narrow<T, CM, false>(a, s, blocks, st);
+}
+
+// returns the number of workgroups, which have left that many partial sums
+template <class T>
+unsigned launch_loss(const LossArgs& a, const Heads& h, hipStream_t st)
+{
+    Small s;
+    // LDS for four waves' heads and gradients must fit a CU
+    const size_t lds = 4 * (size_t)(h.n * WAVE * sizeof(HeadBox) + WAVE * h.width * sizeof(T) + 16);
+    if (take_small(h, &s) && (!a.grad || lds <= 160 * 1024)) {
+        const unsigned blocks = narrow_blocks(a.rows);
+        s.unit = unit_of(a.logits, h.width * sizeof(T), a.ld * sizeof(T), a.rows);
+        s.unit_ref = unit_of(a.ref, h.width * sizeof(T), a.ld_ref * sizeof(T), a.rows);
+        s.unit_mask = unit_of(a.mask, h.width, h.width, a.rows);
+        const bool wide = ((uintptr_t)a.grad & 15) == 0;
+        const int64_t row = h.width * sizeof(T);
+        s.unit_grad = wide && (row == 16 || row == 32) ? 16 : wide ? -16 : -1;
+        if (h.width <= 8) launch_loss_narrow<T, 8>(a, s, blocks, st);
+        else if (h.width <= 16) launch_loss_narrow<T, 16>(a, s, blocks, st);
+        else if (h.width <= 32) launch_loss_narrow<T, 32>(a, s, blocks, st);
+        else launch_loss_narrow<T, 48>(a, s, blocks, st);
+        return blocks;
+    }
+    const unsigned blocks = (unsigned)blocks_for(a.rows);
     if (h.width >= 1024) hipLaunchKernelGGL((loss_rows_kernel<T, 256>), dim3(blocks), dim3(256), 0, st, a, h);
     else hipLaunchKernelGGL((loss_rows_kernel<T, 64>), dim3(blocks), dim3(64), 0, st, a, h);
+    return blocks;
 }
 
 gw_status check_rows(const Heads& h, int32_t dtype, int64_t rows, const void* logits, int64_t ld,
@@ -467,7 +896,7 @@ gw_status gw_policy_loss(const gw_policy_heads* heads, int32_t dtype, int64_t n_
     a.out = out; a.logp = logp; a.grad = grad;
     a.partial = (double*)workspace;
     if (n_rows == 0) {
-        if (out) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(256), 0, st, a, 0);
+        if (out) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(512), 0, st, a, 0);
         LEARN_LAUNCHED();
         return GW_OK;
     }
@@ -476,13 +905,12 @@ gw_status gw_policy_loss(const gw_policy_heads* heads, int32_t dtype, int64_t n_
         const int64_t blocks = (n_rows + 4095) / 4096;
         a.n_counts = (int32_t)(blocks < COUNT_BLOCKS ? blocks : COUNT_BLOCKS);
         a.counts = counts;
-        hipLaunchKernelGGL(count_kernel, dim3(a.n_counts), dim3(256), 0, st, valid, n_rows, counts);
+        hipLaunchKernelGGL(count_kernel, dim3(a.n_counts), dim3(256), 0, st, valid, n_rows,
+                           (int)(((uintptr_t)valid & 15) == 0), counts);
     }
-    const unsigned blocks = (unsigned)blocks_for(n_rows);
-    if (dtype == GW_T_F32) launch_loss<float>(a, h, blocks, st);
-    else if (dtype == GW_T_F16) launch_loss<f16>(a, h, blocks, st);
-    else launch_loss<bf16>(a, h, blocks, st);
-    if (out && blocks > 1) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(256), 0, st, a, (int)blocks);
+    const unsigned blocks = dtype == GW_T_F32 ? launch_loss<float>(a, h, st)
+                          : dtype == GW_T_F16 ? launch_loss<f16>(a, h, st) : launch_loss<bf16>(a, h, st);
+    if (out && blocks > 1) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(512), 0, st, a, (int)blocks);
     LEARN_LAUNCHED();
     return GW_OK;
 }
