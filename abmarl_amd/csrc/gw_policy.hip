@@ -3,6 +3,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "gw_learn.hpp"
 
 static thread_local char g_err[512];
@@ -289,7 +291,7 @@ __device__ inline void block_sums(const LossArgs& a, double* s)
 // reduction crosses lanes, and the memory sees each value once.  A choice that
 // does not exist holds NO_CHOICE, whose exponential is 0.
 constexpr int NARROW = 48;
-constexpr float NO_CHOICE = -1e30f;
+constexpr float NO_CHOICE = -3.2e38f;           // (nobody masks by this number)
 
 struct Small {
     int32_t n, act_dim, width, owned;           // owned: every action column has a head
@@ -336,6 +338,11 @@ __device__ inline float exp_of(float x)
     if constexpr (sizeof(T) == 4) return expf(x);
     return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
 }
+
+// 1/x and the logarithm of sums of exponentials (from 1 to the width): the
+// hardware's, an ulp or two off
+__device__ inline float rcp_of(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ inline float log_of(float x) { return __builtin_amdgcn_logf(x) * 0.69314718055994530942f; }
 
 __device__ inline bool bit(uint64_t b, int j) { return b >> j & 1; }
 
@@ -402,9 +409,9 @@ __global__ __launch_bounds__(256) void sample_narrow_kernel(SampleArgs a, Small 
             at = better ? v[j] : at;
             if (bit(h.ends, j)) {
                 const bool some = sum != 0.f;
-                const float log_s = some ? logf(sum) : 0.f;
+                const float log_s = some ? log_of(sum) : 0.f;
                 logp += some ? (double)at - (double)log_s : 0.;
-                entropy += some ? log_s - t / sum : 0.f;
+                entropy += some ? log_s - t * rcp_of(sum) : 0.f;
                 if (there) act[h.slot[d]] = h.low[d] + (choice < 0 ? 0 : choice - first);
                 sum = t = 0.f;
                 best = NEG_INF;
@@ -478,10 +485,10 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
             }
             if (bit(h.ends, j)) {
                 const bool some = s != 0.f, some_ref = REF && some && sr != 0.f;
-                const float inv = some ? 1.f / s : 0.f, log_s = some ? logf(s) : 0.f, ts = t * inv;
-                const float inv_r = some_ref ? 1.f / sr : 0.f;
+                const float inv = some ? rcp_of(s) : 0.f, log_s = some ? log_of(s) : 0.f, ts = t * inv;
+                const float inv_r = some_ref ? rcp_of(sr) : 0.f;
                 entropy += log_s - ts;
-                if (some_ref) kl += u * inv_r + (log_s - logf(sr));
+                if (some_ref) kl += u * inv_r + log_of(s * inv_r);
                 possible &= found || !some;
                 logp += found ? (double)at - (double)log_s : 0.;
                 if (GRAD) boxes[d * WAVE + lane] = make_float4(inv, ts, inv_r, __int_as_float(found ? first + (int)chosen : -1));
@@ -515,7 +522,8 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
                     b = -beta * q.z;
                     place = __float_as_int(q.w);
                 }
-                float g = e[j] * fmaf(a1, x[j], a0);
+                // (e x is 0 for choices far below, where a1 x may overflow)
+                float g = fmaf(a1, e[j] * x[j], e[j] * a0);
                 if constexpr (REF) g = fmaf(b, y[j], g);
                 g += place == j ? pull : 0.f;
                 x[j] = valid && x[j] != NO_CHOICE ? g : 0.f;
@@ -535,6 +543,366 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
     }
     if (!a.out) return;
     block_sums<4>(a, sums);
+}
+
+// --------------------------------------------------------- one wide head
+// A group of lanes a row: L neighbouring lanes of a wave (several rows a
+// wave), or (L = 0) a workgroup of up to 1024 threads.  Each lane holds V
+// pieces of 16 bytes of the row in registers, so the maximum, the sums and
+// the gradient read the memory once; the gradient makes the exponentials again
+// (kept, they would take twice the row's registers and half the waves).
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+__device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <class T, int V, int L>
+struct WideRow {
+    static constexpr int PER = 16 / sizeof(T), WORD = 4 / sizeof(T);
+    uint32_t w[V * 4];                          // 16-bit logits stay two a register
+
+    // Piece k of this lane is piece at(k) of the row.  The row's last piece is
+    // read so that it ends with the row: what it shares with the piece before it
+    // is marked as no choice, as is a piece behind the row.
+    static __device__ int at(int k) { return L ? k * L + (threadIdx.x & (L ? L - 1 : 0)) : k * (int)blockDim.x + (int)threadIdx.x; }
+    static __device__ int start(int k, int width) { return at(k) * PER < width - PER ? at(k) * PER : width - PER; }
+    // pieces that some lane of this wave has
+    static __device__ int pieces(int width)
+    {
+        const int step = L ? L : (int)blockDim.x, first = L ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63);
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < V; k++) n += (first + k * step) * PER < width ? 1 : 0;
+        return n;
+    }
+
+    __device__ float get(int k, int e) const
+    {
+        const uint32_t u = w[k * 4 + e / WORD];
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, u);
+        else if constexpr (__is_same(T, bf16)) return __builtin_bit_cast(float, e & 1 ? u & 0xffff0000u : u << 16);
+        else return (float)__builtin_bit_cast(f16, (uint16_t)(e & 1 ? u >> 16 : u));
+    }
+    __device__ void none(int k, int e)
+    {
+        constexpr uint32_t inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, bf16) ? 0xff80u : 0xfc00u;
+        uint32_t& u = w[k * 4 + e / WORD];
+        if constexpr (sizeof(T) == 4) u = inf;
+        else u = e & 1 ? (u & 0xffffu) | inf << 16 : (u & 0xffff0000u) | inf;
+    }
+    __device__ void load(const T* row, int width, int n)
+    {
+#pragma unroll
+        for (int k = 0; k < V; k++)
+            if (k < n) __builtin_memcpy(&w[k * 4], row + start(k, width), 16);   // rows may lie anywhere
+    }
+    __device__ void ends(int width, int n)
+    {
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            const int over = at(k) * PER - start(k, width);
+            if (k < n && over > 0)
+#pragma unroll
+                for (int e = 0; e < PER; e++)
+                    if (e < over) none(k, e);
+        }
+    }
+    __device__ void mask(const uint8_t* row, int width, int n)
+    {
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            if (k >= n) continue;
+            uint8_t m[PER];
+            __builtin_memcpy(m, row + start(k, width), PER);
+#pragma unroll
+            for (int e = 0; e < PER; e++)
+                if (!m[e]) none(k, e);
+        }
+    }
+    // choices that the other row has not are none here
+    __device__ void only(const WideRow& o, int n)
+    {
+#pragma unroll
+        for (int k = 0; k < V; k++)
+            if (k < n)
+#pragma unroll
+                for (int e = 0; e < PER; e++)
+                    if (o.get(k, e) == NEG_INF) none(k, e);
+    }
+    // the largest logit, and the smallest (-inf: some choice does not exist)
+    __device__ void range(float& hi, float& lo, int n) const
+    {
+        hi = NEG_INF;
+        lo = -NEG_INF;
+#pragma unroll
+        for (int k = 0; k < V; k++)
+            if (k < n)
+#pragma unroll
+                for (int e = 0; e < PER; e++) {
+                    hi = fmaxf(hi, get(k, e));
+                    lo = fminf(lo, get(k, e));
+                }
+    }
+    // (logit - top) log2(e).  PLAIN: every choice exists and all are of ordinary
+    // size: one fma; its rounding of `top` is common to all choices and to
+    // their sum, so it cancels
+    template <bool PLAIN>
+    __device__ float less(int k, int e, float top) const
+    {
+        const float z = get(k, e);
+        if constexpr (PLAIN) return fmaf(z, LOG2E, -top * LOG2E);
+        // a choice 1e30 below the best (masked by its type's lowest value) is as far as any
+        const float x = (z - top) * LOG2E;
+        return z == NEG_INF ? NO_CHOICE : x < -1e30f ? -1e30f : x;
+    }
+    // what was made of the row before is not to be kept beside it: it is made again
+    __device__ void forget()
+    {
+#pragma unroll
+        for (int i = 0; i < V * 4; i++) asm volatile("" : "+v"(w[i]));
+    }
+};
+
+// sums or maxima of M values over a row's lanes
+template <int L, int M, class Op>
+__device__ inline void over_group(float* v, float (*box)[16], Op op)
+{
+#pragma unroll
+    for (int o = (L ? L : WAVE) / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < M; i++) v[i] = op(v[i], __shfl_xor(v[i], o));
+    if constexpr (L == 0) {
+        const int waves = (int)blockDim.x / WAVE;
+        if (waves == 1) return;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < M; i++) box[i][threadIdx.x >> 6] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < M; i++) {
+            float t = box[i][0];
+            for (int w = 1; w < waves; w++) t = op(t, box[i][w]);
+            v[i] = t;
+        }
+    }
+}
+
+struct OneHead { int32_t width, low, slot, act_dim; };
+
+// where a row's lanes are, and which rows they take
+template <int L>
+struct Rows {
+    static constexpr int PER_BLOCK = L ? 256 / (L ? L : 1) : 1;
+    static __device__ int64_t first() { return L ? (int64_t)blockIdx.x * PER_BLOCK + threadIdx.x / (L ? L : 1) : blockIdx.x; }
+    static __device__ bool leader() { return L ? (threadIdx.x & (L ? L - 1 : 0)) == 0 : threadIdx.x == 0; }
+};
+
+template <class T, int V, int L>
+__global__ __launch_bounds__(L ? 256 : 1024) void sample_wide_kernel(SampleArgs a, OneHead h)
+{
+    __shared__ float box[2][16];
+    __shared__ float best_s[16];
+    __shared__ int best_i[16];
+    typedef WideRow<T, V, L> Row;
+    const int64_t step = (int64_t)gridDim.x * Rows<L>::PER_BLOCK;
+    // (a wave's rows go on together: a row behind the last is the last again)
+    for (int64_t r0 = (int64_t)blockIdx.x * Rows<L>::PER_BLOCK; r0 < a.rows; r0 += step) {
+        const int64_t mine = r0 + (L ? threadIdx.x / (L ? L : 1) : 0), row = mine < a.rows ? mine : a.rows - 1;
+        Row z;
+        const int pieces = Row::pieces(h.width);
+        z.load((const T*)a.logits + row * a.ld, h.width, pieces);
+        if (a.mask) z.mask(a.mask + row % a.mask_rows * h.width, h.width, pieces);
+        z.ends(h.width, pieces);
+        float best = NEG_INF;
+        int choice = INT32_MAX;
+        const float* noise = a.noise + row * h.width;
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            if (k >= pieces) continue;
+            const int j = Row::start(k, h.width);
+            float n[Row::PER];
+            if (a.noise) __builtin_memcpy(n, noise + j, sizeof(n));
+            else
+#pragma unroll
+                for (int e = 0; e < Row::PER; e++) n[e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < Row::PER; e++) {
+                const float v = z.get(k, e), s = v + n[e];
+                const bool better = v != NEG_INF && (s > best || (choice == INT32_MAX && s == best));
+                best = better ? s : best;
+                choice = better ? j + e : choice;
+            }
+        }
+        float m[1], low;
+        z.range(m[0], low, pieces);
+        z.forget();
+        const bool whole = low > -1e30f;
+        over_group<L, 1>(m, box, [](float p, float q) { return fmaxf(p, q); });
+        const float top = m[0] == NEG_INF ? 0.f : m[0];
+        float q[2] = {0.f, 0.f};
+        const auto sum = [&](auto plain) {
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                if (k >= pieces) continue;
+#pragma unroll
+                for (int e = 0; e < Row::PER; e++) {
+                    const float x = z.template less<decltype(plain)::value>(k, e, top), ex = exp2_of(x);
+                    q[0] += ex;
+                    q[1] += ex * x;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        if (__all(whole && fabsf(top) < 1e30f)) sum(std::true_type{});
+        else sum(std::false_type{});
+        q[1] *= LN2;
+        over_group<L, 2>(q, box, [](float p, float r) { return p + r; });
+#pragma unroll
+        for (int o = (L ? L : WAVE) / 2; o > 0; o >>= 1) {
+            const float s = __shfl_xor(best, o);
+            const int i = __shfl_xor(choice, o);
+            if (s > best || (s == best && i < choice)) { best = s; choice = i; }
+        }
+        if constexpr (L == 0) {
+            const int waves = (int)blockDim.x / WAVE;
+            if (waves > 1) {
+                __syncthreads();
+                if ((threadIdx.x & 63) == 0) { best_s[threadIdx.x >> 6] = best; best_i[threadIdx.x >> 6] = choice; }
+                __syncthreads();
+                for (int w = 0; w < waves; w++)
+                    if (best_s[w] > best || (best_s[w] == best && best_i[w] < choice)) { best = best_s[w]; choice = best_i[w]; }
+            }
+        }
+        if (!Rows<L>::leader() || mine >= a.rows) continue;
+        const bool some = q[0] != 0.f;
+        const int c = choice == INT32_MAX ? 0 : choice;
+        int32_t* act = a.actions + row * h.act_dim;
+        for (int i = 0; i < h.act_dim; i++) act[i] = i == h.slot ? h.low + c : 0;
+        const float log_s = some ? log_of(q[0]) : 0.f;
+        if (a.logp)
+            a.logp[row] = some ? (float)((double)((float)((const T*)a.logits)[row * a.ld + c] - top) - (double)log_s) : 0.f;
+        if (a.entropy) a.entropy[row] = some ? log_s - q[1] * rcp_of(q[0]) : 0.f;
+    }
+}
+
+template <class T, int V, int L, bool REF, bool GRAD>
+__global__ __launch_bounds__(L ? 256 : 1024) void loss_wide_kernel(LossArgs a, OneHead h)
+{
+    __shared__ float box[4][16];
+    typedef WideRow<T, V, L> Row;
+    constexpr int PER = Row::PER;
+    double sums[N_SUMS] = {0., 0., 0., 0., 0.};
+    float scale = 0.f;
+    if (GRAD) scale = a.scale * (a.upstream ? *a.upstream : 1.f) * inverse_rows(a);
+    const int64_t step = (int64_t)gridDim.x * Rows<L>::PER_BLOCK;
+    for (int64_t r0 = (int64_t)blockIdx.x * Rows<L>::PER_BLOCK; r0 < a.rows; r0 += step) {
+        const int64_t mine = r0 + (L ? threadIdx.x / (L ? L : 1) : 0), row = mine < a.rows ? mine : a.rows - 1;
+        const bool valid = mine < a.rows && (!a.valid || a.valid[row]);
+        const T* zrow = (const T*)a.logits + row * a.ld;
+        const uint8_t* mask = a.mask ? a.mask + row % a.mask_rows * h.width : nullptr;
+        T* grad = GRAD ? (T*)a.grad + row * h.width : nullptr;
+        Row z, r;
+        const int pieces = Row::pieces(h.width);
+        z.load(zrow, h.width, pieces);
+        if constexpr (REF) r.load((const T*)a.ref + row * a.ld_ref, h.width, pieces);
+        const int c = a.actions[row * h.act_dim + h.slot] - h.low;
+        const bool inside = (uint32_t)c < (uint32_t)h.width;
+        const float zc = inside && (!mask || mask[c]) ? (float)zrow[c] : NEG_INF;
+        if (mask) z.mask(mask, h.width, pieces);
+        z.ends(h.width, pieces);
+        float m[2] = {NEG_INF, NEG_INF}, q[4] = {0.f, 0.f, 0.f, 0.f}, low, low_r = 0.f;
+        z.range(m[0], low, pieces);
+        if constexpr (REF) {
+            if (__any(low == NEG_INF)) r.only(z, pieces);
+            r.range(m[1], low_r, pieces);
+            r.forget();
+        }
+        z.forget();
+        over_group<L, REF ? 2 : 1>(m, box, [](float p, float o) { return fmaxf(p, o); });
+        const float top = m[0] == NEG_INF ? 0.f : m[0], top_r = m[1] == NEG_INF ? 0.f : m[1];
+        // (by waves: most rows are plain but for the pieces behind their ends)
+        const bool plain_wave = __all(low > -1e30f && low_r > -1e30f && fabsf(top) < 1e30f && fabsf(top_r) < 1e30f);
+        const auto sum = [&](auto plain) {
+            constexpr bool PLAIN = decltype(plain)::value;
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                if (k >= pieces) continue;
+#pragma unroll
+                for (int e = 0; e < PER; e++) {
+                    const float x = z.template less<PLAIN>(k, e, top), ex = exp2_of(x);
+                    q[0] += ex;
+                    q[1] += ex * x;
+                    if constexpr (REF) {
+                        const float y = r.template less<PLAIN>(k, e, top_r), ey = exp2_of(y);
+                        q[2] += ey;
+                        q[3] += ey * (y - x);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        if (plain_wave) sum(std::true_type{});
+        else sum(std::false_type{});
+        over_group<L, REF ? 4 : 2>(q, box, [](float p, float o) { return p + o; });
+        const bool some = q[0] != 0.f, some_ref = REF && some && q[2] != 0.f;
+        const float inv = some ? rcp_of(q[0]) : 0.f, log_s = some ? log_of(q[0]) : 0.f, ts = q[1] * inv;
+        const float inv_r = some_ref ? rcp_of(q[2]) : 0.f;
+        const float kl = some_ref ? q[3] * inv_r * LN2 + log_of(q[0] * inv_r) : 0.f;
+        const bool found = some && zc != NEG_INF;
+        // as the sums have it: with the rounding of top
+        const float xc = fabsf(top) < 1e30f && zc > -1e30f ? fmaf(zc, LOG2E, -top * LOG2E) : (zc - top) * LOG2E;
+        const double logp = found ? (double)(xc * LN2) - (double)log_s : 0.;
+        const RowLoss got = row_loss(a, row, logp, found || !some, kl, log_s - ts * LN2);
+        if (Rows<L>::leader() && mine < a.rows) {
+            if (a.logp) a.logp[row] = valid ? got.logp : 0.f;
+            if (valid) {
+                sums[S_PG] += got.pg; sums[S_KL] += got.kl; sums[S_H] += got.entropy;
+                sums[S_CLIP] += got.clipped ? 1. : 0.; sums[S_COUNT] += 1.;
+            }
+        }
+        if constexpr (GRAD) {
+            z.forget();
+            if constexpr (REF) r.forget();
+            // e/S ((beta - pull) + eta (x - T/S)) - beta er/Sr, and pull at the choice
+            // (log p + H = x - T/S)
+            const float pull = got.pull * scale, eta = a.entropy * scale * LN2, beta = a.kl * scale;
+            const float a1 = eta * inv, a0 = inv * ((some_ref ? beta : 0.f) - pull - eta * ts), b = -beta * inv_r;
+            const auto walk = [&](auto plain) {
+                constexpr bool PLAIN = decltype(plain)::value;
+#pragma unroll
+                for (int k = 0; k < V; k++) {
+                    if (k >= pieces) continue;
+                    const int j = Row::start(k, h.width), own = Row::at(k) * PER;
+                    float g[PER];
+#pragma unroll
+                    for (int e = 0; e < PER; e++) {
+                        const float x = z.template less<PLAIN>(k, e, top);
+                        g[e] = exp2_of(x) * fmaf(a1, x, a0);
+                        if constexpr (REF) g[e] = fmaf(b, exp2_of(r.template less<PLAIN>(k, e, top_r)), g[e]);
+                        if (!PLAIN) g[e] = valid && x != NO_CHOICE ? g[e] : 0.f;
+                    }
+                    if (found && valid && (uint32_t)(c - j) < (uint32_t)PER && c >= own)
+#pragma unroll
+                        for (int e = 0; e < PER; e++) g[e] += j + e == c ? pull : 0.f;
+                    T t[PER];
+#pragma unroll
+                    for (int e = 0; e < PER; e++) t[e] = (T)g[e];
+                    if (mine < a.rows) {
+                        if (PLAIN || own == j) __builtin_memcpy(grad + j, t, 16);
+                        else
+#pragma unroll
+                            for (int e = 0; e < PER; e++)
+                                if (j + e >= own) grad[j + e] = t[e];
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            if (plain_wave && __all(valid)) walk(std::true_type{});
+            else walk(std::false_type{});
+        }
+    }
+    if (!a.out) return;
+    if constexpr (L > 0) block_sums<4>(a, sums);
+    else if (threadIdx.x < WAVE) block_sums<1>(a, sums);
 }
 
 // One row by one workgroup of G threads, as sample_rows_kernel: maximum,
@@ -601,7 +969,7 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                     sr = grp.sum(sr);
                     u = grp.sum(u);
                     inv_r = 1.f / sr;
-                    kl += u * inv_r + (log_s - logf(sr));
+                    kl += u * inv_r + logf(s * inv_r);
                 }
                 const int c = act[h.slot[d]] - h.low[d];
                 const float v = c >= 0 && c < hi - lo ? logit_at(z, mask, lo + c) : NEG_INF;
@@ -666,25 +1034,28 @@ __global__ __launch_bounds__(256) void count_kernel(const uint8_t* valid, int64_
     if (threadIdx.x == 0) counts[blockIdx.x] = box[0] + box[1] + box[2] + box[3];
 }
 
-// the blocks' partial sums, added in a fixed order, to the loss and its parts
-__global__ __launch_bounds__(512) void finish_kernel(LossArgs a, int blocks)
+// the blocks' partial sums, added in a fixed order, to the loss and its parts:
+// two waves for each of the sums, eight loads in flight a lane
+__global__ __launch_bounds__(2 * N_SUMS * WAVE) void finish_kernel(LossArgs a, int blocks)
 {
-    __shared__ double box[8];
-    __shared__ double total[N_SUMS];
-    for (int k = 0; k < N_SUMS; k++) {
-        double s = 0.;
-        for (int b = threadIdx.x; b < blocks; b += 512) s += a.partial[(int64_t)k * blocks + b];
-        s = wave_sum(s);
-        if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = s;
-        __syncthreads();
-        if (threadIdx.x == 0)
-            total[k] = ((box[0] + box[1]) + (box[2] + box[3])) + ((box[4] + box[5]) + (box[6] + box[7]));
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) write_out(a, total);
+    __shared__ double box[2 * N_SUMS];
+    const int wave = threadIdx.x >> 6, k = wave >> 1;
+    const double* p = a.partial + (int64_t)k * blocks;
+    double s[8] = {0., 0., 0., 0., 0., 0., 0., 0.};
+    for (int b = threadIdx.x & (2 * WAVE - 1); b < blocks; b += 16 * WAVE)
+#pragma unroll
+        for (int i = 0; i < 8; i++) s[i] += b + i * 2 * WAVE < blocks ? p[b + i * 2 * WAVE] : 0.;
+    const double t = wave_sum(((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])));
+    if ((threadIdx.x & 63) == 0) box[wave] = t;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    double total[N_SUMS];
+    for (int i = 0; i < N_SUMS; i++) total[i] = box[2 * i] + box[2 * i + 1];
+    write_out(a, total);
 }
 
 constexpr int MAX_BLOCKS = 8192;
+constexpr int64_t NARROW_BLOCKS = 2048;         // 256 CUs, 8 workgroups of 4 waves each
 
 // the host's heads, checked, as the kernels take them
 gw_status take_heads(const gw_policy_heads* p, Heads* h)
@@ -736,8 +1107,6 @@ bool take_small(const Heads& h, Small* s)
     return true;
 }
 
-constexpr int64_t NARROW_BLOCKS = 2048;         // 256 CUs, 8 workgroups of 4 waves each
-
 unsigned narrow_blocks(int64_t rows)
 {
     const int64_t tiles = (rows + 4 * WAVE - 1) / (4 * WAVE);
@@ -750,9 +1119,55 @@ void launch_sample_narrow(const SampleArgs& a, const Small& s, hipStream_t st)
     hipLaunchKernelGGL((sample_narrow_kernel<T, CM>), dim3(narrow_blocks(a.rows)), dim3(256), 0, st, a, s);
 }
 
+// How a wide head's rows are shared out, or false where registers do not hold
+// them: pieces of 16 bytes, one or (from 256 on) four a lane; fewer than a
+// wave's lanes a row where the row has fewer pieces.
+struct WideSplit { int v, lanes, threads; };
+
+bool take_wide(const Heads& h, int size, WideSplit* w)
+{
+    if (h.n != 1 || h.width <= NARROW) return false;
+    const int pieces = (h.width * size + 15) / 16;
+    w->v = pieces > 64 ? 4 : 1;
+    const int lanes = (pieces + w->v - 1) / w->v;
+    if (lanes > 1024) return false;
+    w->lanes = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : lanes <= 64 ? 64 : 0;
+    w->threads = w->lanes ? 256 : (lanes + 63) / 64 * 64;
+    return true;
+}
+
+unsigned wide_blocks(const WideSplit& w, int64_t rows)
+{
+    // as many as the device holds at once, a few times over
+    const int64_t per = w.lanes ? 256 / w.lanes : 1, need = (rows + per - 1) / per;
+    const int64_t most = w.lanes ? NARROW_BLOCKS : 4096;
+    return (unsigned)(need < most ? need : most);
+}
+
+template <class T, int V>
+void launch_sample_wide(const SampleArgs& a, const OneHead& o, const WideSplit& w, hipStream_t st)
+{
+    const dim3 grid(wide_blocks(w, a.rows)), block(w.threads);
+    if constexpr (V == 1) {
+        if (w.lanes == 8) hipLaunchKernelGGL((sample_wide_kernel<T, V, 8>), grid, block, 0, st, a, o);
+        if (w.lanes == 16) hipLaunchKernelGGL((sample_wide_kernel<T, V, 16>), grid, block, 0, st, a, o);
+    }
+    if (w.lanes == 32) hipLaunchKernelGGL((sample_wide_kernel<T, V, 32>), grid, block, 0, st, a, o);
+    if (w.lanes == 64) hipLaunchKernelGGL((sample_wide_kernel<T, V, 64>), grid, block, 0, st, a, o);
+    if constexpr (V > 1)
+        if (w.lanes == 0) hipLaunchKernelGGL((sample_wide_kernel<T, V, 0>), grid, block, 0, st, a, o);
+}
+
 template <class T>
 void launch_sample(const SampleArgs& a, const Heads& h, hipStream_t st)
 {
+    WideSplit w;
+    if (take_wide(h, sizeof(T), &w)) {
+        const OneHead o{h.width, h.low[0], h.slot[0], h.act_dim};
+        if (w.v == 1) launch_sample_wide<T, 1>(a, o, w, st);
+        else launch_sample_wide<T, 4>(a, o, w, st);
+        return;
+    }
     Small s;
     if (take_small(h, &s)) {
         s.unit = unit_of(a.logits, h.width * sizeof(T), a.ld * sizeof(T), a.rows);
@@ -790,10 +1205,34 @@ void launch_loss_narrow(const LossArgs& a, const Small& s, unsigned blocks, hipS
     else launch_loss_narrow<T, CM, false>(a, s, blocks, st);
 }
 
+template <class T, int V, int L>
+void launch_loss_wide(const LossArgs& a, const OneHead& o, unsigned blocks, int threads, hipStream_t st)
+{
+    const dim3 grid(blocks), block(threads);
+    if (a.ref && a.grad) hipLaunchKernelGGL((loss_wide_kernel<T, V, L, true, true>), grid, block, 0, st, a, o);
+    else if (a.ref) hipLaunchKernelGGL((loss_wide_kernel<T, V, L, true, false>), grid, block, 0, st, a, o);
+    else if (a.grad) hipLaunchKernelGGL((loss_wide_kernel<T, V, L, false, true>), grid, block, 0, st, a, o);
+    else hipLaunchKernelGGL((loss_wide_kernel<T, V, L, false, false>), grid, block, 0, st, a, o);
+}
+
 // returns the number of workgroups, which have left that many partial sums
 template <class T>
 unsigned launch_loss(const LossArgs& a, const Heads& h, hipStream_t st)
 {
+    WideSplit w;
+    if (take_wide(h, sizeof(T), &w)) {
+        const OneHead o{h.width, h.low[0], h.slot[0], h.act_dim};
+        const unsigned blocks = wide_blocks(w, a.rows);
+        if (w.v == 1) {
+            if (w.lanes == 8) launch_loss_wide<T, 1, 8>(a, o, blocks, w.threads, st);
+            else if (w.lanes == 16) launch_loss_wide<T, 1, 16>(a, o, blocks, w.threads, st);
+            else if (w.lanes == 32) launch_loss_wide<T, 1, 32>(a, o, blocks, w.threads, st);
+            else launch_loss_wide<T, 1, 64>(a, o, blocks, w.threads, st);
+        } else if (w.lanes == 32) launch_loss_wide<T, 4, 32>(a, o, blocks, w.threads, st);
+        else if (w.lanes == 64) launch_loss_wide<T, 4, 64>(a, o, blocks, w.threads, st);
+        else launch_loss_wide<T, 4, 0>(a, o, blocks, w.threads, st);
+        return blocks;
+    }
     Small s;
     // LDS for four waves' heads and gradients must fit a CU
     const size_t lds = 4 * (size_t)(h.n * WAVE * sizeof(HeadBox) + WAVE * h.width * sizeof(T) + 16);
@@ -896,7 +1335,7 @@ gw_status gw_policy_loss(const gw_policy_heads* heads, int32_t dtype, int64_t n_
     a.out = out; a.logp = logp; a.grad = grad;
     a.partial = (double*)workspace;
     if (n_rows == 0) {
-        if (out) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(512), 0, st, a, 0);
+        if (out) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(2 * N_SUMS * WAVE), 0, st, a, 0);
         LEARN_LAUNCHED();
         return GW_OK;
     }
@@ -910,7 +1349,7 @@ gw_status gw_policy_loss(const gw_policy_heads* heads, int32_t dtype, int64_t n_
     }
     const unsigned blocks = dtype == GW_T_F32 ? launch_loss<float>(a, h, st)
                           : dtype == GW_T_F16 ? launch_loss<f16>(a, h, st) : launch_loss<bf16>(a, h, st);
-    if (out && blocks > 1) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(512), 0, st, a, (int)blocks);
+    if (out && blocks > 1) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(2 * N_SUMS * WAVE), 0, st, a, (int)blocks);
     LEARN_LAUNCHED();
     return GW_OK;
 }

@@ -78,14 +78,18 @@ def _at(t):
 
 
 def _tensor(t, name, dtypes, device=None, shape=None):
-    """t is a contiguous tensor of one of the dtypes, there, of that shape."""
-    _need(isinstance(t, torch.Tensor), f"{name}: a tensor is needed, not {type(t).__name__}")
-    _need(t.dtype in dtypes, f"{name}: {t.dtype}, not one of {', '.join(str(d) for d in dtypes)}")
-    if shape is not None:
-        _need(t.shape == shape, f"{name}: shape {tuple(t.shape)}, not {tuple(shape)}")
-    _need(t.is_contiguous(), f"{name}: must be contiguous")
-    if device is not None:
-        _need(t.device == device, f"{name}: on {t.device}, not on {device}")
+    """t is a contiguous tensor of one of the dtypes, there, of that shape
+    (this runs in every call: messages are made only for errors)."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: a tensor is needed, not {type(t).__name__}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: {t.dtype}, not one of {', '.join(str(d) for d in dtypes)}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, not {tuple(shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name}: on {t.device}, not on {device}")
     return t
 
 
@@ -97,9 +101,12 @@ _I32 = (torch.int32,)
 def _rows(t, name, width):
     """(rows, elements between rows) of a matrix of logits: the last dimension
     side by side, the others one stride."""
-    _need(isinstance(t, torch.Tensor), f"{name}: a tensor is needed, not {type(t).__name__}")
-    _need(t.dtype in _DTYPES, f"{name}: {t.dtype}, not float32, float16 or bfloat16")
-    _need(t.dim() >= 1 and t.shape[-1] == width, f"{name}: shape {tuple(t.shape)}, not (..., {width})")
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: a tensor is needed, not {type(t).__name__}")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name}: {t.dtype}, not float32, float16 or bfloat16")
+    if t.dim() < 1 or t.shape[-1] != width:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, not (..., {width})")
     if t.is_contiguous():
         return t.numel() // width, width
     _need(t.stride(-1) == 1 or width == 1, f"{name}: the choices of a row must lie side by side")
@@ -140,8 +147,8 @@ class _On:
     __slots__ = ('guard', 'stream')
 
     def __init__(self, device):
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-        self.stream = torch.cuda.current_stream(device).cuda_stream
+        self.guard = None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+        self.stream = torch._C._cuda_getCurrentRawStream(device.index)
 
     def __enter__(self):
         if self.guard is not None:
@@ -252,15 +259,17 @@ class _PolicyLoss(torch.autograd.Function):
                      out=out, logp=logp)
         ctx.save_for_backward(logits, actions, advantage, old_logp, ref, valid, mask, at, out)
         ctx.rest = heads, args, kl_coef, entropy_coef
-        loss = out[0].clone()
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(out, logp)
-        return loss, out, logp
+        return out.select(0, 0).detach(), out, logp
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_loss, _out, _logp):
         logits, actions, advantage, old_logp, ref, valid, mask, at, out = ctx.saved_tensors
         heads, args, kl_coef, entropy_coef = ctx.rest
+        if d_loss is None:
+            return (None,) * 12
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         _launch_loss(logits, actions, advantage, old_logp, ref, valid, heads, args, kl_coef, entropy_coef,
                      upstream=d_loss.contiguous(), grad=grad, denominator_at=out[5])
