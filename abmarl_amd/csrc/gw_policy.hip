@@ -168,12 +168,11 @@ struct RowLoss {
 
 // (L is a sum of numbers near its own size: in double its difference to
 // old_logp, which is near 0, is exact to the heads' own errors)
-__device__ inline RowLoss row_loss(const LossArgs& a, int64_t row, double logp, bool possible, float kl, float entropy)
+__device__ inline RowLoss row_loss(const LossArgs& a, float adv, float old, double logp, bool possible, float kl, float entropy)
 {
     RowLoss r;
     r.logp = possible ? (float)logp : NEG_INF;
-    const float adv = a.advantage[row];
-    const float ratio = possible ? expf((float)(logp - (double)a.old_logp[row])) : 0.f;
+    const float ratio = possible ? expf((float)(logp - (double)old)) : 0.f;
     const float clamped = fminf(fmaxf(ratio, a.lo), a.hi);
     const float free = ratio * adv, held = (ratio != ratio ? ratio : clamped) * adv;
     r.clipped = held < free;
@@ -284,6 +283,11 @@ __device__ inline void block_sums(const LossArgs& a, double* s)
         for (int k = 0; k < N_SUMS; k++) a.partial[(int64_t)k * gridDim.x + blockIdx.x] = s[k];
 }
 
+// Softmax sums are made in powers of two: the hardware's 2^x, 1/x and log2 x
+// are an ulp off, where float32's own rounding of x (up to 2^-24 |x|) is no less
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+__device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // ------------------------------------------------------------- narrow rows
 // A thread a row, the whole row in registers (CM: the width, rounded up).
 // Where the heads begin and end is uniform, so the sweeps over a row are
@@ -296,38 +300,98 @@ constexpr float NO_CHOICE = -3.2e38f;           // (nobody masks by this number)
 struct Small {
     int32_t n, act_dim, width, owned;           // owned: every action column has a head
     uint64_t starts, ends;                      // bit j: choice j is a head's first, last
-    int32_t low[NARROW];
-    int16_t slot[NARROW];
+    int32_t low[NARROW + 3];                    // (read in fours)
+    int16_t slot[NARROW + 3];
+    uint8_t first[NARROW + 3], size[NARROW + 3];  // a head's first choice, how many
     int32_t unit, unit_ref, unit_mask, unit_grad, unit_noise;  // bytes that a row's loads and stores may take at once
 };
 
-template <class T, int CM, class W>
-__device__ inline void load_units(const T* row, int width, float* v)
-{
-    constexpr int PER = sizeof(W) / sizeof(T);
-    W w[CM / PER];
-#pragma unroll
-    for (int u = 0; u < CM / PER; u++)
-        if (u * PER < width) w[u] = ((const W*)row)[u];
-#pragma unroll
-    for (int u = 0; u < CM / PER; u++) {
-        T t[PER];
-        __builtin_memcpy(t, &w[u], sizeof(W));
-#pragma unroll
-        for (int e = 0; e < PER; e++) v[u * PER + e] = u * PER + e < width ? (float)t[e] : NEG_INF;
+// A wave's 64 rows: a uniform first one and the lane's own behind it (the last
+// row again for lanes behind it)
+struct Tile {
+    int64_t base;
+    uint32_t l;
+    bool there;
+    __device__ Tile(int64_t tile, int64_t rows, int lane) : base(tile * WAVE)
+    {
+        const int64_t left = rows - 1 - base;
+        there = lane <= left;
+        l = there ? (uint32_t)lane : (uint32_t)left;
     }
-}
+};
 
-// a row of `width` <= CM values, -inf behind them
-template <class T, int CM>
-__device__ inline void load_row(const T* row, int width, int unit, float* v)
-{
-    if constexpr (CM * sizeof(T) % 16 == 0) {
-        if (unit == 16) return load_units<T, CM, uint4>(row, width, v);
+// The heads' ends are tested dozens of times a row.  Without this the
+// compiler keeps every test's outcome over all rows, in more scalar
+// registers than there are.
+struct Bounds {
+    uint64_t starts, ends;
+    int32_t width, n, unit, unit_ref;
+    __device__ explicit Bounds(const Small& h)
+        : starts(h.starts), ends(h.ends), width(h.width), n(h.n), unit(h.unit), unit_ref(h.unit_ref)
+    {
+        asm volatile("" : "+s"(starts), "+s"(ends), "+s"(width), "+s"(n), "+s"(unit), "+s"(unit_ref));
     }
-    if (unit >= 8) load_units<T, CM, uint2>(row, width, v);
-    else if (unit >= 4) load_units<T, CM, uint32_t>(row, width, v);
-    else load_units<T, CM, T>(row, width, v);
+};
+
+// A row of up to CM values as they lie in memory, so that the loads of the
+// next tile can be in flight while this one is worked on
+template <class T, int CM>
+struct Packed {
+    static constexpr int WORDS = CM * (int)sizeof(T) / 4, PER = 4 / (int)sizeof(T);
+    uint32_t w[WORDS];
+
+    template <class W>
+    __device__ void load_units(const char* at, int width)
+    {
+        constexpr int N = sizeof(W) / 4;
+#pragma unroll
+        for (int u = 0; u < WORDS / N; u++)
+            if (u * N * PER < width) {
+                const W t = ((const W*)at)[u];
+                __builtin_memcpy(&w[u * N], &t, sizeof(W));
+            }
+    }
+    // `first`: elements from the uniform `rows` to this lane's row; unit: see Small
+    __device__ void load(const T* rows, uint32_t first, int width, int unit)
+    {
+        const char* at = (const char*)rows + first * (uint32_t)sizeof(T);
+        if constexpr (WORDS % 4 == 0) {
+            if (unit == 16) return load_units<uint4>(at, width);
+        }
+        if constexpr (WORDS % 2 == 0) {
+            if (unit >= 8) return load_units<uint2>(at, width);
+        }
+        if (unit >= 4) return load_units<uint32_t>(at, width);
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+            T t[PER];
+#pragma unroll
+            for (int e = 0; e < PER; e++) t[e] = i * PER + e < width ? ((const T*)at)[i * PER + e] : (T)0.f;
+            __builtin_memcpy(&w[i], t, 4);
+        }
+    }
+    // -inf behind the row
+    __device__ void get(int width, float* v) const
+    {
+#pragma unroll
+        for (int j = 0; j < CM; j++) {
+            const uint32_t u = w[j / PER];
+            float f;
+            if constexpr (sizeof(T) == 4) f = __builtin_bit_cast(float, u);
+            else if constexpr (sizeof(T) == 1) f = (float)(u >> 8 * (j % 4) & 0xffu);
+            else if constexpr (__is_same(T, bf16)) f = __builtin_bit_cast(float, j & 1 ? u & 0xffff0000u : u << 16);
+            else f = (float)__builtin_bit_cast(f16, (uint16_t)(j & 1 ? u >> 16 : u));
+            v[j] = j < width ? f : NEG_INF;
+        }
+    }
+};
+
+template <class T, int CM>
+__device__ inline void load_row(const T* rows, uint32_t first, int width, int unit, float* v)
+{
+    Packed<T, CM> p;
+    p.load(rows, first, width, unit);
+    p.get(width, v);
 }
 
 // e^x: for 16-bit logits the hardware's 2^x, 2^-20 near for |x| < 16 and far
@@ -348,7 +412,7 @@ __device__ inline bool bit(uint64_t b, int j) { return b >> j & 1; }
 
 // v[j] less its head's maximum (0 where a head has no choice; NaN stays)
 template <int CM>
-__device__ inline void subtract_max(const Small& h, float* v)
+__device__ inline void subtract_max(const Bounds& h, float* v)
 {
     float m[CM];
 #pragma unroll
@@ -363,13 +427,14 @@ __device__ inline void subtract_max(const Small& h, float* v)
 
 // masked choices of the row to -inf; row r uses mask row r % mask_rows
 template <int CM>
-__device__ inline void apply_mask(const uint8_t* mask, int64_t mask_rows, int64_t tile_row, int lane, int width, int unit,
-                                  float* v)
+__device__ inline void apply_mask(const uint8_t* mask, int64_t mask_rows, int64_t tile_row, uint32_t l, int width,
+                                  int unit, float* v)
 {
-    int64_t r = tile_row % mask_rows + lane;
+    const int64_t first = tile_row % mask_rows;
+    int64_t r = first + l;
     r = mask_rows >= WAVE ? (r >= mask_rows ? r - mask_rows : r) : (int64_t)((uint32_t)r % (uint32_t)mask_rows);
     float m[CM];
-    load_row<uint8_t, CM>(mask + r * width, width, unit, m);
+    load_row<uint8_t, CM>(mask + r * width, 0, width, unit, m);
 #pragma unroll
     for (int j = 0; j < CM; j++) v[j] = m[j] == 0.f ? NEG_INF : v[j];
 }
@@ -380,23 +445,26 @@ __global__ __launch_bounds__(256) void sample_narrow_kernel(SampleArgs a, Small 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int64_t tiles = (a.rows + WAVE - 1) / WAVE, waves = (int64_t)gridDim.x * 4;
     for (int64_t tile = (int64_t)blockIdx.x * 4 + wave; tile < tiles; tile += waves) {
-        const int64_t base = tile * WAVE, row = base + lane < a.rows ? base + lane : a.rows - 1;
-        const bool there = base + lane < a.rows;
+        const Tile at_row(tile, a.rows, lane);
+        const bool there = at_row.there;
+        const Bounds b(h);
         float v[CM], s[CM];
-        load_row<T, CM>((const T*)a.logits + row * a.ld, h.width, h.unit, v);
-        if (a.noise) load_row<float, CM>(a.noise + row * h.width, h.width, h.unit_noise, s);
-        if (a.mask) apply_mask<CM>(a.mask, a.mask_rows, base, (int)(row - base), h.width, h.unit_mask, v);
+        load_row<T, CM>((const T*)a.logits + at_row.base * a.ld, at_row.l * (uint32_t)a.ld, h.width, h.unit, v);
+        if (a.noise)
+            load_row<float, CM>(a.noise + at_row.base * h.width, at_row.l * (uint32_t)h.width, h.width, h.unit_noise, s);
+        if (a.mask) apply_mask<CM>(a.mask, a.mask_rows, at_row.base, at_row.l, h.width, h.unit_mask, v);
 #pragma unroll
         for (int j = 0; j < CM; j++) s[j] = a.noise ? v[j] + s[j] : v[j];
         float raw[CM];
 #pragma unroll
         for (int j = 0; j < CM; j++) raw[j] = v[j];
-        subtract_max<CM>(h, v);
+        subtract_max<CM>(b, v);
         float sum = 0.f, t = 0.f, best = NEG_INF, at = __builtin_nanf("");
         int choice = -1, d = 0, first = 0;
         double logp = 0.;
         float entropy = 0.f;
-        int32_t* act = a.actions + row * h.act_dim;
+        int32_t* acts = a.actions + at_row.base * h.act_dim;
+        const uint32_t act = at_row.l * (uint32_t)h.act_dim;
 #pragma unroll
         for (int j = 0; j < CM; j++) {
             const float e = exp_of<T>(v[j]);
@@ -407,12 +475,12 @@ __global__ __launch_bounds__(256) void sample_narrow_kernel(SampleArgs a, Small 
             best = better ? s[j] : best;
             choice = better ? j : choice;
             at = better ? v[j] : at;
-            if (bit(h.ends, j)) {
+            if (bit(b.ends, j)) {
                 const bool some = sum != 0.f;
                 const float log_s = some ? log_of(sum) : 0.f;
                 logp += some ? (double)at - (double)log_s : 0.;
                 entropy += some ? log_s - t * rcp_of(sum) : 0.f;
-                if (there) act[h.slot[d]] = h.low[d] + (choice < 0 ? 0 : choice - first);
+                if (there) acts[act + h.slot[d]] = h.low[d] + (choice < 0 ? 0 : choice - first);
                 sum = t = 0.f;
                 best = NEG_INF;
                 at = __builtin_nanf("");
@@ -426,122 +494,239 @@ __global__ __launch_bounds__(256) void sample_narrow_kernel(SampleArgs a, Small 
             for (int c = 0; c < h.act_dim; c++) {
                 bool has = false;
                 for (int k = 0; k < h.n; k++) has |= h.slot[k] == c;
-                if (!has) act[c] = 0;
+                if (!has) acts[act + c] = 0;
             }
-        if (a.logp) a.logp[row] = (float)logp;
-        if (a.entropy) a.entropy[row] = entropy;
+        if (a.logp) (a.logp + at_row.base)[at_row.l] = (float)logp;
+        if (a.entropy) (a.entropy + at_row.base)[at_row.l] = entropy;
     }
 }
 
-// What the gradient needs of a head again: 1/S, T/S, 1/S of ref, the choice's place
-typedef float4 HeadBox;
+// Logits to (logit - top) log2(e), in place: their heads' tops, or, where no
+// logit of a wave's rows is more than SPAN below its row's largest, the row's
+// (sums of at least 2^(-1.5 SPAN) lose nothing by it): one fma a choice.
+constexpr float SPAN = 16.f;
+
+template <int CM>
+__device__ inline bool row_span(const float* v, int width, float& top)
+{
+    float low = -NEG_INF;
+    top = NEG_INF;
+#pragma unroll
+    for (int j = 0; j < CM; j++) {
+        top = fmaxf(top, v[j]);
+        low = fminf(low, j < width ? v[j] : -NEG_INF);
+    }
+    return low > top - SPAN && fabsf(top) < 1e30f;
+}
+
+template <int CM>
+__device__ inline void from_row_top(float top, float* v)
+{
+#pragma unroll
+    for (int j = 0; j < CM; j++) v[j] = fmaf(v[j], LOG2E, -top * LOG2E);
+}
+
+template <int CM>
+__device__ inline void from_head_top(const Bounds& h, float* v)
+{
+    float m[CM];
+#pragma unroll
+    for (int j = 0; j < CM; j++) m[j] = j == 0 ? v[0] : fmaxf(v[j], bit(h.starts, j) ? NEG_INF : m[j - 1]);
+    float top = 0.f;
+#pragma unroll
+    for (int j = CM - 1; j >= 0; j--) {
+        if (bit(h.ends, j)) top = m[j] == NEG_INF ? 0.f : m[j];
+        // a choice 1e30 below the best (masked by its type's lowest value) is as far as any
+        const float x = (v[j] - top) * LOG2E;
+        v[j] = v[j] == NEG_INF ? NO_CHOICE : x < -1e30f ? -1e30f : x;
+    }
+}
+
+// The sums of a row's heads lie in LDS, a plane of 64 floats each: every lane
+// reads only what it wrote.  The unrolled sweeps over the choices stay short;
+// what is done once a head is a loop over the heads.
+enum { P_S, P_T, P_AT, P_SR, P_U };             // afterwards 1/S, T/S and 1/S of ref in P_S, P_T, P_SR
 
 template <class T, int CM, bool REF, bool GRAD>
 __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
 {
     extern __shared__ float4 lds[];
+    constexpr int PLANES = REF ? 5 : 3;
+    typedef typename std::conditional<(CM > 32), uint64_t, uint32_t>::type Picks;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    // per wave: [heads][64] boxes, then the tile of gradients
+    // per wave: [heads][PLANES][64] sums, then the tile of gradients
     const int tile_bytes = GRAD && h.unit_grad < 0 ? (WAVE * h.width * (int)sizeof(T) + 15) & ~15 : 0;
-    char* mine = (char*)lds + wave * ((GRAD ? h.n * WAVE * (int)sizeof(HeadBox) : 0) + tile_bytes);
-    HeadBox* boxes = (HeadBox*)mine;
-    T* out = (T*)(mine + h.n * WAVE * sizeof(HeadBox));
+    char* mine = (char*)lds + wave * (h.n * PLANES * WAVE * 4 + tile_bytes);
+    float* planes = (float*)mine + lane;
+    T* out = (T*)(mine + h.n * PLANES * WAVE * 4);
     const int64_t tiles = (a.rows + WAVE - 1) / WAVE, waves = (int64_t)gridDim.x * 4;
     float step = 0.f;
     if (GRAD) step = a.scale * (a.upstream ? *a.upstream : 1.f) * inverse_rows(a);
     double sums[N_SUMS] = {0., 0., 0., 0., 0.};
-    for (int64_t tile = (int64_t)blockIdx.x * 4 + wave; tile < tiles; tile += waves) {
-        const int64_t base = tile * WAVE, row = base + lane < a.rows ? base + lane : a.rows - 1;
-        const bool there = base + lane < a.rows, valid = there && (!a.valid || a.valid[row]);
-        float x[CM], y[REF ? CM : 1], e[CM];
-        load_row<T, CM>((const T*)a.logits + row * a.ld, h.width, h.unit, x);
-        if constexpr (REF) load_row<T, CM>((const T*)a.ref + row * a.ld_ref, h.width, h.unit_ref, y);
-        if (a.mask) apply_mask<CM>(a.mask, a.mask_rows, base, (int)(row - base), h.width, h.unit_mask, x);
-        if constexpr (REF) {
+    int64_t clipped = 0, count = 0;
+    // what a tile reads, loaded a tile ahead
+    struct {
+        Packed<T, CM> z, r;
+        float adv, old;
+        int32_t act[4];
+        uint8_t valid;
+    } next;
+    const auto fetch = [&](int64_t tile) {
+        const Tile at_row(tile, a.rows, lane);
+        const int64_t base = at_row.base;
+        const uint32_t l = at_row.l;
+        const Bounds heads(h);
+        next.z.load((const T*)a.logits + base * a.ld, l * (uint32_t)a.ld, heads.width, heads.unit);
+        if constexpr (REF) next.r.load((const T*)a.ref + base * a.ld_ref, l * (uint32_t)a.ld_ref, heads.width, heads.unit_ref);
+        const int32_t* acts = a.actions + base * h.act_dim;
 #pragma unroll
-            for (int j = 0; j < CM; j++) y[j] = x[j] == NEG_INF ? NEG_INF : y[j];
-            subtract_max<CM>(h, y);
+        for (int d = 0; d < 4; d++) next.act[d] = acts[l * (uint32_t)h.act_dim + h.slot[d < heads.n ? d : 0]];
+        next.adv = (a.advantage + base)[l];
+        next.old = (a.old_logp + base)[l];
+        next.valid = a.valid ? (a.valid + base)[l] : 1;
+    };
+    int64_t tile = (int64_t)blockIdx.x * 4 + wave;
+    if (tile < tiles) fetch(tile);
+    for (; tile < tiles; tile += waves) {
+        const Tile at_row(tile, a.rows, lane);
+        const int64_t base = at_row.base;
+        const uint32_t l = at_row.l;
+        const Bounds heads(h);
+        float x[CM], y[REF ? CM : 1], e[CM];
+        next.z.get(heads.width, x);
+        if constexpr (REF) next.r.get(heads.width, y);
+        const bool there = at_row.there, valid = there && next.valid;
+        const float adv = next.adv, old = next.old;
+        // bit j: choice j is its head's action
+        Picks picks = 0;
+        for (int d = 0; d < heads.n; d += 4) {
+            if (d > 0) {
+                const int32_t* acts = a.actions + base * h.act_dim;
+#pragma unroll
+                for (int k = 0; k < 4; k++) next.act[k] = acts[l * (uint32_t)h.act_dim + h.slot[d + k < heads.n ? d + k : 0]];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t c = (uint32_t)next.act[k] - (uint32_t)h.low[d + k];
+                picks |= d + k < heads.n && c < (uint32_t)h.size[d + k] ? (Picks)1 << (h.first[d + k] + (int)c) : 0;
+            }
         }
-        subtract_max<CM>(h, x);
-        const int32_t* act = a.actions + row * h.act_dim;
-        float s = 0.f, t = 0.f, sr = 0.f, u = 0.f, at = 0.f, kl = 0.f, entropy = 0.f;
-        double logp = 0.;
-        bool possible = true, found = false;
-        int d = 0, first = 0;
-        uint32_t chosen = (uint32_t)act[h.slot[0]] - (uint32_t)h.low[0];
+        if (tile + waves < tiles) fetch(tile + waves);
+        if (a.mask) apply_mask<CM>(a.mask, a.mask_rows, base, l, h.width, h.unit_mask, x);
+        float top, top_r = 0.f;
+        bool near = row_span<CM>(x, heads.width, top);
+        if constexpr (REF) near &= row_span<CM>(y, heads.width, top_r);
+        if (__all(near || !valid)) {
+            from_row_top<CM>(top, x);
+            if constexpr (REF) from_row_top<CM>(top_r, y);
+        } else {
+            if constexpr (REF) {
+#pragma unroll
+                for (int j = 0; j < CM; j++) y[j] = x[j] == NEG_INF ? NEG_INF : y[j];
+                from_head_top<CM>(heads, y);
+            }
+            from_head_top<CM>(heads, x);
+        }
+        float s = 0.f, t = 0.f, at = 0.f, sr = 0.f, u = 0.f;
+        float* plane = planes;
 #pragma unroll
         for (int j = 0; j < CM; j++) {
-            e[j] = exp_of<T>(x[j]);
-            s += e[j];
-            t += e[j] * x[j];
-            const bool it = (uint32_t)(j - first) == chosen && x[j] != NO_CHOICE;
-            at = it ? x[j] : at;
-            found |= it;
+            const float on = __uint_as_float(0x3f800000u * (1u - (uint32_t)(heads.starts >> j & 1)));
+            e[j] = exp2_of(x[j]);
+            s = fmaf(on, s, e[j]);
+            t = fmaf(on, t, e[j] * x[j]);
+            const uint32_t pick = 0u - (uint32_t)(picks >> j & 1);
+            at = fmaf(on, at, __uint_as_float(pick & __float_as_uint(x[j])));
             if constexpr (REF) {
-                const float er = exp_of<T>(y[j]);
-                sr += er;
-                u += er * (y[j] - x[j]);
+                const float er = exp2_of(y[j]);
+                sr = fmaf(on, sr, er);
+                u = fmaf(on, u, er * (y[j] - x[j]));
                 y[j] = er;
             }
-            if (bit(h.ends, j)) {
-                const bool some = s != 0.f, some_ref = REF && some && sr != 0.f;
-                const float inv = some ? rcp_of(s) : 0.f, log_s = some ? log_of(s) : 0.f, ts = t * inv;
-                const float inv_r = some_ref ? rcp_of(sr) : 0.f;
-                entropy += log_s - ts;
-                if (some_ref) kl += u * inv_r + log_of(s * inv_r);
-                possible &= found || !some;
-                logp += found ? (double)at - (double)log_s : 0.;
-                if (GRAD) boxes[d * WAVE + lane] = make_float4(inv, ts, inv_r, __int_as_float(found ? first + (int)chosen : -1));
-                s = t = sr = u = 0.f;
-                found = false;
-                first = j + 1;
-                d++;
-                if (d < h.n) chosen = (uint32_t)act[h.slot[d]] - (uint32_t)h.low[d];
+            if (bit(heads.ends, j)) {
+                plane[P_S * WAVE] = s;
+                plane[P_T * WAVE] = t;
+                plane[P_AT * WAVE] = at;
+                if constexpr (REF) {
+                    plane[P_SR * WAVE] = sr;
+                    plane[P_U * WAVE] = u;
+                }
+                plane += PLANES * WAVE;
             }
         }
-        const RowLoss r = row_loss(a, row, logp, possible, kl, entropy);
-        if (a.logp && there) a.logp[row] = valid ? r.logp : 0.f;
-        if (valid) {
-            sums[S_PG] += r.pg; sums[S_KL] += r.kl; sums[S_H] += r.entropy;
-            sums[S_CLIP] += r.clipped ? 1. : 0.; sums[S_COUNT] += 1.;
+        float kl = 0.f, entropy = 0.f;
+        double logp = 0.;
+        bool possible = true;
+        plane = planes;
+        for (int d = 0; d < h.n; d++, plane += PLANES * WAVE) {
+            const float sd = plane[P_S * WAVE], atd = plane[P_AT * WAVE];
+            const bool some = sd != 0.f;
+            const float inv = some ? rcp_of(sd) : 0.f, log_s = some ? log_of(sd) : 0.f, ts = plane[P_T * WAVE] * inv;
+            const Picks of = ((Picks)~(Picks)0 >> (8 * (int)sizeof(Picks) - h.size[d])) << h.first[d];
+            const bool found = (picks & of) != 0 && atd > -1e38f;
+            entropy += log_s - ts * LN2;
+            possible &= found || !some;
+            logp += found && some ? (double)(atd * LN2) - (double)log_s : 0.;
+            if constexpr (REF) {
+                const float srd = plane[P_SR * WAVE];
+                const bool some_ref = some && srd != 0.f;
+                const float inv_r = some_ref ? rcp_of(srd) : 0.f;
+                kl += some_ref ? plane[P_U * WAVE] * inv_r * LN2 + log_of(sd * inv_r) : 0.f;
+                if (GRAD) plane[P_SR * WAVE] = inv_r;
+            }
+            if (GRAD) {
+                plane[P_S * WAVE] = inv;
+                plane[P_T * WAVE] = ts;
+            }
+        }
+        const RowLoss r = row_loss(a, adv, old, logp, possible, kl, entropy);
+        if (a.logp && there) (a.logp + base)[l] = valid ? r.logp : 0.f;
+        if (a.out) {
+            sums[S_PG] += valid ? r.pg : 0.f;
+            sums[S_KL] += valid ? r.kl : 0.f;
+            sums[S_H] += valid ? r.entropy : 0.f;
+            clipped += __popcll(__ballot(valid && r.clipped));
+            count += __popcll(__ballot(valid));
         }
         if constexpr (GRAD) {
-            const float pull = r.pull * step, eta = a.entropy * step, beta = a.kl * step;
+            // g = e/S ((beta - pull) + eta (x - T/S)) - beta er/Sr, and pull at the choice:
+            // log p + H = x - T/S
+            const float pull = r.pull * step, eta = a.entropy * step * LN2, beta = a.kl * step;
             float a0 = 0.f, a1 = 0.f, b = 0.f;
-            int place = -1;
-            wave_sync();
+            const Bounds again(h);
+            asm volatile("" : "+v"(picks));                // tested again, not kept choice by choice
+            plane = planes;
 #pragma unroll
-            for (int j = CM - 1; j >= 0; j--) {
-                if (bit(h.ends, j)) {
-                    d--;
-                    const HeadBox q = boxes[d * WAVE + lane];
-                    // g = e/S ((beta - pull) + eta (x - T/S)) - beta er/Sr, and pull at the choice:
-                    // log p + H = x - T/S
-                    a1 = eta * q.x;
-                    a0 = q.x * ((q.z != 0.f ? beta : 0.f) - pull - eta * q.y);
-                    b = -beta * q.z;
-                    place = __float_as_int(q.w);
+            for (int j = 0; j < CM; j++) {
+                if (bit(again.starts, j)) {
+                    const float inv = plane[P_S * WAVE], ts = plane[P_T * WAVE], inv_r = REF ? plane[P_SR * WAVE] : 0.f;
+                    a1 = eta * inv;
+                    a0 = inv * ((inv_r != 0.f ? beta : 0.f) - pull - eta * ts);
+                    b = -beta * inv_r;
+                    plane += PLANES * WAVE;
                 }
                 // (e x is 0 for choices far below, where a1 x may overflow)
                 float g = fmaf(a1, e[j] * x[j], e[j] * a0);
                 if constexpr (REF) g = fmaf(b, y[j], g);
-                g += place == j ? pull : 0.f;
+                const uint32_t pick = 0u - (uint32_t)(picks >> j & 1);
+                g += __uint_as_float(pick & __float_as_uint(pull));
                 x[j] = valid && x[j] != NO_CHOICE ? g : 0.f;
             }
             T* grad = (T*)a.grad + base * h.width;
             if (h.unit_grad > 0) {
                 // rows of one or two 16-byte pieces: straight from the registers
-                if (there) store_row<T, CM>(grad + lane * h.width, h.width, x);
+                if (there) store_row<T, CM>(grad + l * (uint32_t)again.width, again.width, x);
             } else {
-                write_tile<T, CM>(out + lane * h.width, h.width, x);
+                write_tile<T, CM>(out + lane * again.width, again.width, x);
                 wave_sync();
                 const int64_t rows = a.rows - base < WAVE ? a.rows - base : WAVE;
-                copy_tile<T>(out, grad, (int)rows * h.width, h.unit_grad == -16, lane);
+                copy_tile<T>(out, grad, (int)rows * again.width, h.unit_grad == -16, lane);
                 wave_sync();
             }
         }
     }
     if (!a.out) return;
+    if (lane == 0) { sums[S_CLIP] = (double)clipped; sums[S_COUNT] = (double)count; }
     block_sums<4>(a, sums);
 }
 
@@ -551,9 +736,6 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
 // pieces of 16 bytes of the row in registers, so the maximum, the sums and
 // the gradient read the memory once; the gradient makes the exponentials again
 // (kept, they would take twice the row's registers and half the waves).
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-__device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
-
 template <class T, int V, int L>
 struct WideRow {
     static constexpr int PER = 16 / sizeof(T), WORD = 4 / sizeof(T);
@@ -851,7 +1033,7 @@ __global__ __launch_bounds__(L ? 256 : 1024) void loss_wide_kernel(LossArgs a, O
         // as the sums have it: with the rounding of top
         const float xc = fabsf(top) < 1e30f && zc > -1e30f ? fmaf(zc, LOG2E, -top * LOG2E) : (zc - top) * LOG2E;
         const double logp = found ? (double)(xc * LN2) - (double)log_s : 0.;
-        const RowLoss got = row_loss(a, row, logp, found || !some, kl, log_s - ts * LN2);
+        const RowLoss got = row_loss(a, a.advantage[row], a.old_logp[row], logp, found || !some, kl, log_s - ts * LN2);
         if (Rows<L>::leader() && mine < a.rows) {
             if (a.logp) a.logp[row] = valid ? got.logp : 0.f;
             if (valid) {
@@ -980,7 +1162,7 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                 hm[d] = m; hls[d] = log_s; hinv[d] = inv; hh[d] = ent; hrm[d] = mr; hrinv[d] = inv_r;
             }
         }
-        const RowLoss r = row_loss(a, row, logp, possible, kl, entropy);
+        const RowLoss r = row_loss(a, a.advantage[row], a.old_logp[row], logp, possible, kl, entropy);
         if (tid == 0) {
             if (a.logp) a.logp[row] = r.logp;
             sums[S_PG] += r.pg; sums[S_KL] += r.kl; sums[S_H] += r.entropy;
@@ -1093,9 +1275,10 @@ int unit_of(const void* p, int64_t row_bytes, int64_t apart, int64_t rows)
 }
 
 // the narrow kernels' heads, or false if the rows are not narrow
-bool take_small(const Heads& h, Small* s)
+bool take_small(const Heads& h, int64_t ld, int64_t ld_ref, Small* s)
 {
-    if (h.width > NARROW) return false;
+    // (a tile's offsets are 32 bits)
+    if (h.width > NARROW || ld > (1 << 22) || ld_ref > (1 << 22)) return false;
     *s = Small{};
     s->n = h.n; s->act_dim = h.act_dim; s->width = h.width; s->owned = h.n == h.act_dim;
     for (int d = 0; d < h.n; d++) {
@@ -1103,6 +1286,8 @@ bool take_small(const Heads& h, Small* s)
         s->ends |= UINT64_C(1) << (h.off[d + 1] - 1);
         s->low[d] = h.low[d];
         s->slot[d] = h.slot[d];
+        s->first[d] = (uint8_t)h.off[d];
+        s->size[d] = (uint8_t)(h.off[d + 1] - h.off[d]);
     }
     return true;
 }
@@ -1169,7 +1354,7 @@ void launch_sample(const SampleArgs& a, const Heads& h, hipStream_t st)
         return;
     }
     Small s;
-    if (take_small(h, &s)) {
+    if (take_small(h, a.rows > 1 ? a.ld : 0, 0, &s)) {
         s.unit = unit_of(a.logits, h.width * sizeof(T), a.ld * sizeof(T), a.rows);
         s.unit_noise = unit_of(a.noise, h.width * 4, h.width * 4, a.rows);
         s.unit_mask = unit_of(a.mask, h.width, h.width, a.rows);
@@ -1187,14 +1372,15 @@ void launch_sample(const SampleArgs& a, const Heads& h, hipStream_t st)
 template <class T, int CM, bool REF>
 void launch_loss_narrow(const LossArgs& a, const Small& s, unsigned blocks, hipStream_t st)
 {
-    size_t lds = 0;
+    const size_t sums = (size_t)s.n * (REF ? 5 : 3) * WAVE * 4;
     if (a.grad) {
-        lds = 4 * ((size_t)s.n * WAVE * sizeof(HeadBox) + (s.unit_grad < 0 ? (WAVE * s.width * sizeof(T) + 15) & ~(size_t)15 : 0));
-        const void* k = (const void*)loss_narrow_kernel<T, CM, REF, true>;
-        if (lds > 64 * 1024) (void)hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        const size_t lds = 4 * (sums + (s.unit_grad < 0 ? (WAVE * s.width * sizeof(T) + 15) & ~(size_t)15 : 0));
+        if (lds > 64 * 1024)
+            (void)hipFuncSetAttribute((const void*)loss_narrow_kernel<T, CM, REF, true>,
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         hipLaunchKernelGGL((loss_narrow_kernel<T, CM, REF, true>), dim3(blocks), dim3(256), lds, st, a, s);
     } else {
-        hipLaunchKernelGGL((loss_narrow_kernel<T, CM, REF, false>), dim3(blocks), dim3(256), lds, st, a, s);
+        hipLaunchKernelGGL((loss_narrow_kernel<T, CM, REF, false>), dim3(blocks), dim3(256), 4 * sums, st, a, s);
     }
 }
 
@@ -1234,9 +1420,9 @@ unsigned launch_loss(const LossArgs& a, const Heads& h, hipStream_t st)
         return blocks;
     }
     Small s;
-    // LDS for four waves' heads and gradients must fit a CU
-    const size_t lds = 4 * (size_t)(h.n * WAVE * sizeof(HeadBox) + WAVE * h.width * sizeof(T) + 16);
-    if (take_small(h, &s) && (!a.grad || lds <= 160 * 1024)) {
+    // LDS for four waves' heads and gradients: two workgroups must fit a CU
+    const size_t lds = 4 * (size_t)(h.n * (a.ref ? 5 : 3) * WAVE * 4 + WAVE * h.width * sizeof(T) + 16);
+    if (take_small(h, a.rows > 1 ? a.ld : 0, a.rows > 1 ? a.ld_ref : 0, &s) && lds <= 160 * 1024) {
         const unsigned blocks = narrow_blocks(a.rows);
         s.unit = unit_of(a.logits, h.width * sizeof(T), a.ld * sizeof(T), a.rows);
         s.unit_ref = unit_of(a.ref, h.width * sizeof(T), a.ld_ref * sizeof(T), a.rows);
