@@ -93,6 +93,8 @@ def _tensor(t, name, dtypes, device=None, shape=None):
     return t
 
 
+_INF = float('inf')
+_FLOATS = tuple(_DTYPES)
 _BYTES = (torch.uint8, torch.bool)
 _F32 = (torch.float32,)
 _I32 = (torch.int32,)
@@ -128,10 +130,10 @@ def _mask(t, shape, device):
     if t is None:
         return None, 0
     k = t.dim() if isinstance(t, torch.Tensor) else -1
-    _need(1 <= k <= len(shape) and t.shape == shape[len(shape) - k:] or
-          k == 2 and len(shape) == 2 and t.shape[1] == shape[1] and t.shape[0] >= 1 and shape[0] % t.shape[0] == 0,
-          f"choice_mask: shape {tuple(t.shape) if k >= 0 else type(t).__name__} is not that of the logits' last "
-          f"dimensions {tuple(shape)}")
+    if not (1 <= k <= len(shape) and t.shape == shape[len(shape) - k:] or
+            k == 2 and len(shape) == 2 and t.shape[1] == shape[1] and t.shape[0] >= 1 and shape[0] % t.shape[0] == 0):
+        raise ValueError(f"choice_mask: shape {tuple(t.shape) if k >= 0 else type(t).__name__} is not that of the "
+                         f"logits' last dimensions {tuple(shape)}")
     _tensor(t, 'choice_mask', _BYTES, device)
     return t, t.numel() // shape[-1]
 
@@ -141,23 +143,30 @@ def _gpu(device):
         raise RuntimeError("the policy operators need a ROCm GPU (no CPU fallback).")
 
 
-class _On:
-    """The tensors' device is the current one while the work is put on its
-    current stream (a context only where it is not already)."""
-    __slots__ = ('guard', 'stream')
+_libs = None
 
-    def __init__(self, device):
-        self.guard = None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
-        self.stream = torch._C._cuda_getCurrentRawStream(device.index)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
+def _lib():
+    global _libs
+    if _libs is None:
+        _libs = _native.learn_lib()
+    return _libs
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+
+_device_now, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _call(fn, device, *args):
+    """fn(*args, stream) with the tensors' device the current one, on that
+    device's current stream."""
+    i = device.index
+    if _device_now() == i:
+        st = fn(*args, _stream_of(i))
+    else:
+        with torch.cuda.device(i):
+            st = fn(*args, _stream_of(i))
+    if st:
+        _native.check_learn(st, fn.__name__)
 
 
 # ------------------------------------------------------------------ sampling
@@ -189,12 +198,8 @@ def sample_actions(logits, heads, noise=None, choice_mask=None, out=None):
         out = torch.empty(lead + (heads.act_dim,), dtype=torch.int32, device=device)
     logp = torch.empty(lead, dtype=torch.float32, device=device)
     entropy = torch.empty(lead, dtype=torch.float32, device=device)
-    with _On(device) as stream:
-        st = _native.learn_lib().gw_policy_sample(
-            heads._p, _DTYPES[logits.dtype], n, logits.data_ptr(), ld, _at(noise), _at(mask), mask_rows,
-            out.data_ptr(), logp.data_ptr(), entropy.data_ptr(), stream)
-    if st:
-        _native.check_learn(st, 'gw_policy_sample')
+    _call(_lib().gw_policy_sample, device, heads._p, _DTYPES[logits.dtype], n, logits.data_ptr(), ld, _at(noise),
+          _at(mask), mask_rows, out.data_ptr(), logp.data_ptr(), entropy.data_ptr())
     return Sampled(out, logp, entropy)
 
 
@@ -206,8 +211,8 @@ def _loss_args(logits, actions, advantage, old_logp, heads, ref_logits, valid, c
     ld_ref = 0
     if ref_logits is not None:
         _, ld_ref = _rows(ref_logits, 'ref_logits', heads.n_choices)
-        _need(ref_logits.shape == logits.shape and ref_logits.dtype == logits.dtype and ref_logits.device == device,
-              "ref_logits: shape, dtype and device must be the logits'")
+        if ref_logits.shape != logits.shape or ref_logits.dtype != logits.dtype or ref_logits.device != device:
+            raise ValueError("ref_logits: shape, dtype and device must be the logits'")
     _tensor(actions, 'actions', _I32, device, lead + (heads.act_dim,))
     _tensor(advantage, 'advantage', _F32, device, lead)
     _tensor(old_logp, 'old_logp', _F32, device, lead)
@@ -216,38 +221,36 @@ def _loss_args(logits, actions, advantage, old_logp, heads, ref_logits, valid, c
     mask, mask_rows = _mask(choice_mask, logits.shape, device)
     low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
     low, high = float(low), float(high)
-    _need(0 <= low < float('inf') and 0 <= high < float('inf'), f"clip {clip}: finite, not negative")
+    if not (0 <= low < _INF and 0 <= high < _INF):
+        raise ValueError(f"clip {clip}: finite, not negative")
     value, at = 0.0, None
     if isinstance(denominator, torch.Tensor):
         at = _tensor(denominator, 'denominator', _F32, device, torch.Size([]))
     elif denominator is not None:
         value = float(denominator)
         _need(0 < value < float('inf'), f"denominator {denominator}: finite and positive")
-    for name, t in (('ref_logits', ref_logits), ('advantage', advantage), ('old_logp', old_logp)):
-        _need(t is None or not t.requires_grad, f"{name}: no gradient flows to it, detach it")
+    if advantage.requires_grad or old_logp.requires_grad or ref_logits is not None and ref_logits.requires_grad:
+        raise ValueError("advantage, old_logp, ref_logits: no gradient flows to them, detach them")
     return n, ld, ld_ref, mask, mask_rows, low, high, value, at
 
 
 def _finite(name, v):
     v = float(v)
-    _need(abs(v) < float('inf'), f"{name} {v}: must be finite")
+    if not abs(v) < _INF:
+        raise ValueError(f"{name} {v}: must be finite")
     return v
 
 
 def _launch_loss(logits, actions, advantage, old_logp, ref, valid, heads, args, kl_coef, entropy_coef,
                  grad_scale=1.0, upstream=None, out=None, logp=None, grad=None, denominator_at=None):
     n, ld, ld_ref, mask, mask_rows, low, high, value, at = args
-    L = _native.learn_lib()
-    with _On(logits.device) as stream:
-        size = L.gw_policy_loss_workspace(n)
-        work = torch.empty(size, dtype=torch.uint8, device=logits.device)
-        st = L.gw_policy_loss(
-            heads._p, _DTYPES[logits.dtype], n, logits.data_ptr(), ld, _at(ref), ld_ref, actions.data_ptr(),
-            advantage.data_ptr(), old_logp.data_ptr(), _at(valid), _at(mask), mask_rows, low, high, kl_coef,
-            entropy_coef, value, _at(at if denominator_at is None else denominator_at), grad_scale, _at(upstream),
-            _at(out), _at(logp), _at(grad), work.data_ptr(), size, stream)
-    if st:
-        _native.check_learn(st, 'gw_policy_loss')
+    L, device = _lib(), logits.device
+    size = L.gw_policy_loss_workspace(n)
+    work = torch.empty(size, dtype=torch.uint8, device=device)
+    _call(L.gw_policy_loss, device, heads._p, _DTYPES[logits.dtype], n, logits.data_ptr(), ld, _at(ref), ld_ref,
+          actions.data_ptr(), advantage.data_ptr(), old_logp.data_ptr(), _at(valid), _at(mask), mask_rows, low, high,
+          kl_coef, entropy_coef, value, _at(at if denominator_at is None else denominator_at), grad_scale,
+          _at(upstream), _at(out), _at(logp), _at(grad), work.data_ptr(), size)
 
 
 class _PolicyLoss(torch.autograd.Function):
@@ -334,8 +337,8 @@ def _span(shape, t, name):
         return 1
     k = t.dim()
     lead = t.shape[:-1] if k == len(shape) and t.shape[-1] == 1 else t.shape
-    _need(1 <= len(lead) <= len(shape) and lead == shape[:len(lead)],
-          f"{name}: shape {tuple(t.shape)} is neither x's {tuple(shape)} nor the first dimensions of it")
+    if not (1 <= len(lead) <= len(shape) and lead == shape[:len(lead)]):
+        raise ValueError(f"{name}: shape {tuple(t.shape)} is neither x's {tuple(shape)} nor the first dimensions of it")
     n = 1
     for s in shape[len(lead):]:
         n *= s
@@ -345,16 +348,12 @@ def _span(shape, t, name):
 def _launch_recurrence(gate, value, gate_span, x, state, cut, cut_span, reverse, h, last, carry):
     T = x.shape[0]
     n = x.numel() // T if T else last.numel()
-    L = _native.learn_lib()
-    with _On(x.device) as stream:
-        size = L.gw_recurrence_workspace(T, n)
-        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        st = L.gw_recurrence(
-            _DTYPES[x.dtype], _DTYPES[x.dtype if gate is None else gate.dtype], T, n, x.data_ptr(), _at(gate),
-            gate_span, value, _at(cut), cut_span, _at(state), reverse, h.data_ptr(), last.data_ptr(), _at(carry),
-            _at(work), size, stream)
-    if st:
-        _native.check_learn(st, 'gw_recurrence')
+    L, device = _lib(), x.device
+    size = L.gw_recurrence_workspace(T, n)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _call(L.gw_recurrence, device, _DTYPES[x.dtype], _DTYPES[x.dtype if gate is None else gate.dtype], T, n,
+          x.data_ptr(), _at(gate), gate_span, value, _at(cut), cut_span, _at(state), reverse, h.data_ptr(),
+          last.data_ptr(), _at(carry), _at(work), size)
 
 
 class _Recurrence(torch.autograd.Function):
@@ -385,16 +384,12 @@ class _Recurrence(torch.autograd.Function):
             if has_state and ctx.needs_input_grad[2] else None
         dh = None if dh is None else dh.contiguous()
         dlast = None if dlast is None else dlast.contiguous()
-        L = _native.learn_lib()
-        with _On(device) as stream:
-            size = L.gw_recurrence_backward_workspace(T, n, gate_span)
-            work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-            st = L.gw_recurrence_backward(
-                _DTYPES[x.dtype], _DTYPES[x.dtype if gate is None else gate.dtype], T, n, x.data_ptr(), _at(gate),
-                gate_span, value, _at(cut), cut_span, carry.data_ptr(), reverse, _at(dh), _at(dlast), dx.data_ptr(),
-                _at(dgate), _at(dstate), _at(work), size, stream)
-        if st:
-            _native.check_learn(st, 'gw_recurrence_backward')
+        L = _lib()
+        size = L.gw_recurrence_backward_workspace(T, n, gate_span)
+        work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        _call(L.gw_recurrence_backward, device, _DTYPES[x.dtype], _DTYPES[x.dtype if gate is None else gate.dtype], T, n,
+              x.data_ptr(), _at(gate), gate_span, value, _at(cut), cut_span, carry.data_ptr(), reverse, _at(dh),
+              _at(dlast), dx.data_ptr(), _at(dgate), _at(dstate), _at(work), size)
         return dgate, dx, dstate, None, None, None, None, None
 
 
@@ -413,8 +408,9 @@ def linear_recurrence(gate, x, state=None, cut=None, reverse=False):
 
     Differentiable by gate, x and state; a shared gate's gradient is summed
     in a fixed order.  One step (T = 1) is the form for acting."""
-    _need(isinstance(x, torch.Tensor) and x.dim() >= 2, "x: a tensor [steps, ...] is needed")
-    _tensor(x, 'x', tuple(_DTYPES))
+    if not isinstance(x, torch.Tensor) or x.dim() < 2:
+        raise ValueError("x: a tensor [steps, ...] is needed")
+    _tensor(x, 'x', _FLOATS)
     shape, device = x.shape, x.device
     value, gate_span = 0.0, 1
     if isinstance(gate, torch.Tensor):
@@ -465,12 +461,8 @@ def fragment_marks(all_done, steps=None, horizon=0, autoreset='next_step', all_d
     _need(0 <= int(horizon) < 2**31, f"horizon {horizon}")
     _gpu(device)
     marks = torch.empty((K, E), dtype=torch.uint8, device=device)
-    with _On(device) as stream:
-        st = _native.learn_lib().gw_fragment_marks(
-            K, E, all_done.data_ptr(), _at(all_done_before), _at(steps), _at(err), int(horizon),
-            1 if autoreset == 'same_step' else 2, marks.data_ptr(), stream)
-    if st:
-        _native.check_learn(st, 'gw_fragment_marks')
+    _call(_lib().gw_fragment_marks, device, K, E, all_done.data_ptr(), _at(all_done_before), _at(steps), _at(err),
+          int(horizon), 1 if autoreset == 'same_step' else 2, marks.data_ptr())
     return marks
 
 
@@ -493,7 +485,7 @@ def advantages(reward, value, done, marks, live, gamma=0.99, lam=0.95, acts=None
     _need(reward.dim() == 3, f"reward: shape {tuple(reward.shape)}, not (steps, envs, lanes)")
     K, E, A = shape = reward.shape
     device = reward.device
-    _tensor(value, 'value', tuple(_DTYPES), device, torch.Size([K + 1, E, A]))
+    _tensor(value, 'value', _FLOATS, device, torch.Size([K + 1, E, A]))
     _tensor(done, 'done', _BYTES, device, shape)
     _tensor(marks, 'marks', (torch.uint8,), device, torch.Size([K, E]))
     _tensor(live, 'live', _BYTES, device, torch.Size([E, A]))
@@ -504,14 +496,10 @@ def advantages(reward, value, done, marks, live, gamma=0.99, lam=0.95, acts=None
     adv = torch.empty(shape, dtype=torch.float32, device=device)
     target = torch.empty(shape, dtype=torch.float32, device=device)
     valid = torch.empty(shape, dtype=torch.uint8, device=device)
-    L = _native.learn_lib()
-    with _On(device) as stream:
-        size = L.gw_recurrence_workspace(K, E * A)
-        work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        st = L.gw_advantages(
-            _DTYPES[value.dtype], int(reward.dtype == torch.float64), K, E, A, reward.data_ptr(), value.data_ptr(),
-            done.data_ptr(), marks.data_ptr(), live.data_ptr(), _at(acts), gamma, lam, adv.data_ptr(),
-            target.data_ptr(), valid.data_ptr(), _at(work), size, stream)
-    if st:
-        _native.check_learn(st, 'gw_advantages')
+    L = _lib()
+    size = L.gw_recurrence_workspace(K, E * A)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _call(L.gw_advantages, device, _DTYPES[value.dtype], int(reward.dtype == torch.float64), K, E, A, reward.data_ptr(),
+          value.data_ptr(), done.data_ptr(), marks.data_ptr(), live.data_ptr(), _at(acts), gamma, lam, adv.data_ptr(),
+          target.data_ptr(), valid.data_ptr(), _at(work), size)
     return Advantages(adv, target, valid)
