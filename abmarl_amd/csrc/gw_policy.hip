@@ -425,18 +425,19 @@ __device__ inline void subtract_max(const Bounds& h, float* v)
     }
 }
 
-// masked choices of the row to -inf; row r uses mask row r % mask_rows
-template <int CM>
-__device__ inline void apply_mask(const uint8_t* mask, int64_t mask_rows, int64_t tile_row, uint32_t l, int width,
-                                  int unit, float* v)
+// row r uses mask row r % mask_rows
+__device__ inline int64_t mask_row(int64_t mask_rows, int64_t tile_row, uint32_t l)
 {
-    const int64_t first = tile_row % mask_rows;
-    int64_t r = first + l;
-    r = mask_rows >= WAVE ? (r >= mask_rows ? r - mask_rows : r) : (int64_t)((uint32_t)r % (uint32_t)mask_rows);
-    float m[CM];
-    load_row<uint8_t, CM>(mask + r * width, 0, width, unit, m);
+    const int64_t r = tile_row % mask_rows + l;
+    return mask_rows >= WAVE ? (r >= mask_rows ? r - mask_rows : r) : (int64_t)((uint32_t)r % (uint32_t)mask_rows);
+}
+
+// masked choices to -inf
+template <int CM>
+__device__ inline void apply_mask(const Packed<uint8_t, CM>& m, float* v)
+{
 #pragma unroll
-    for (int j = 0; j < CM; j++) v[j] = m[j] == 0.f ? NEG_INF : v[j];
+    for (int j = 0; j < CM; j++) v[j] = (m.w[j / 4] >> 8 * (j % 4) & 0xffu) == 0 ? NEG_INF : v[j];
 }
 
 template <class T, int CM>
@@ -452,7 +453,11 @@ __global__ __launch_bounds__(256) void sample_narrow_kernel(SampleArgs a, Small 
         load_row<T, CM>((const T*)a.logits + at_row.base * a.ld, at_row.l * (uint32_t)a.ld, h.width, h.unit, v);
         if (a.noise)
             load_row<float, CM>(a.noise + at_row.base * h.width, at_row.l * (uint32_t)h.width, h.width, h.unit_noise, s);
-        if (a.mask) apply_mask<CM>(a.mask, a.mask_rows, at_row.base, at_row.l, h.width, h.unit_mask, v);
+        if (a.mask) {
+            Packed<uint8_t, CM> m;
+            m.load(a.mask + mask_row(a.mask_rows, at_row.base, at_row.l) * h.width, 0, h.width, h.unit_mask);
+            apply_mask<CM>(m, v);
+        }
 #pragma unroll
         for (int j = 0; j < CM; j++) s[j] = a.noise ? v[j] + s[j] : v[j];
         float raw[CM];
@@ -519,11 +524,25 @@ __device__ inline bool row_span(const float* v, int width, float& top)
     return low > top - SPAN && fabsf(top) < 1e30f;
 }
 
+// the same over the choices that exist
 template <int CM>
+__device__ inline bool some_span(const float* v, float top)
+{
+    float low = -NEG_INF;
+#pragma unroll
+    for (int j = 0; j < CM; j++) low = fminf(low, v[j] == NEG_INF ? -NEG_INF : v[j]);
+    return top == NEG_INF || (low > top - SPAN && fabsf(top) < 1e30f);
+}
+
+template <int CM, bool ALL>
 __device__ inline void from_row_top(float top, float* v)
 {
+    const float t = ALL || top != NEG_INF ? -top * LOG2E : 0.f;
 #pragma unroll
-    for (int j = 0; j < CM; j++) v[j] = fmaf(v[j], LOG2E, -top * LOG2E);
+    for (int j = 0; j < CM; j++) {
+        const float x = fmaf(v[j], LOG2E, t);
+        v[j] = ALL ? x : v[j] == NEG_INF ? NO_CHOICE : x;
+    }
 }
 
 template <int CM>
@@ -567,6 +586,7 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
     // what a tile reads, loaded a tile ahead
     struct {
         Packed<T, CM> z, r;
+        Packed<uint8_t, CM> mask;
         float adv, old;
         int32_t act[4];
         uint8_t valid;
@@ -584,6 +604,7 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
         next.adv = (a.advantage + base)[l];
         next.old = (a.old_logp + base)[l];
         next.valid = a.valid ? (a.valid + base)[l] : 1;
+        if (a.mask) next.mask.load(a.mask + mask_row(a.mask_rows, base, l) * heads.width, 0, heads.width, h.unit_mask);
     };
     int64_t tile = (int64_t)blockIdx.x * 4 + wave;
     if (tile < tiles) fetch(tile);
@@ -611,21 +632,29 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
                 picks |= d + k < heads.n && c < (uint32_t)h.size[d + k] ? (Picks)1 << (h.first[d + k] + (int)c) : 0;
             }
         }
+        if (a.mask) apply_mask<CM>(next.mask, x);
         if (tile + waves < tiles) fetch(tile + waves);
-        if (a.mask) apply_mask<CM>(a.mask, a.mask_rows, base, l, h.width, h.unit_mask, x);
         float top, top_r = 0.f;
         bool near = row_span<CM>(x, heads.width, top);
         if constexpr (REF) near &= row_span<CM>(y, heads.width, top_r);
         if (__all(near || !valid)) {
-            from_row_top<CM>(top, x);
-            if constexpr (REF) from_row_top<CM>(top_r, y);
+            from_row_top<CM, true>(top, x);
+            if constexpr (REF) from_row_top<CM, true>(top_r, y);
         } else {
+            near = some_span<CM>(x, top);
             if constexpr (REF) {
 #pragma unroll
                 for (int j = 0; j < CM; j++) y[j] = x[j] == NEG_INF ? NEG_INF : y[j];
-                from_head_top<CM>(heads, y);
+                (void)row_span<CM>(y, heads.width, top_r);
+                near &= some_span<CM>(y, top_r);
             }
-            from_head_top<CM>(heads, x);
+            if (__all(near || !valid)) {
+                from_row_top<CM, false>(top, x);
+                if constexpr (REF) from_row_top<CM, false>(top_r, y);
+            } else {
+                from_head_top<CM>(heads, x);
+                if constexpr (REF) from_head_top<CM>(heads, y);
+            }
         }
         float s = 0.f, t = 0.f, at = 0.f, sr = 0.f, u = 0.f;
         float* plane = planes;
@@ -694,7 +723,10 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
             const float pull = r.pull * step, eta = a.entropy * step * LN2, beta = a.kl * step;
             float a0 = 0.f, a1 = 0.f, b = 0.f;
             const Bounds again(h);
-            asm volatile("" : "+v"(picks));                // tested again, not kept choice by choice
+            // products and tests are made again, not kept for every choice
+            asm volatile("" : "+v"(picks));
+#pragma unroll
+            for (int j = 0; j < CM; j++) asm volatile("" : "+v"(x[j]));
             plane = planes;
 #pragma unroll
             for (int j = 0; j < CM; j++) {
