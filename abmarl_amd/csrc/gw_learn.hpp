@@ -37,24 +37,24 @@ typedef __bf16 bf16;
 constexpr float NEG_INF = -__builtin_inff();
 
 // the larger of two, NaN if either is: a NaN logit must not vanish in a maximum
-__device__ inline float max_nan(float a, float b) { return (b > a || b != b) ? b : a; }
+__device__ __forceinline__ float max_nan(float a, float b) { return (b > a || b != b) ? b : a; }
 
 // what a wave's lanes have written to LDS is there for its other lanes
-__device__ inline void wave_sync()
+__device__ __forceinline__ void wave_sync()
 {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
 
 template <class V>
-__device__ inline V wave_sum(V v)
+__device__ __forceinline__ V wave_sum(V v)
 {
 #pragma unroll
     for (int o = WAVE / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
 
-__device__ inline float wave_max_nan(float v)
+__device__ __forceinline__ float wave_max_nan(float v)
 {
 #pragma unroll
     for (int o = WAVE / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor(v, o));

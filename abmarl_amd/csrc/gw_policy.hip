@@ -52,7 +52,7 @@ enum { S_PG, S_KL, S_H, S_CLIP, S_COUNT, N_SUMS };
 template <int G>
 struct Group {
     float* box;                                 // G / 64 floats of LDS
-    __device__ float max(float v)
+    __device__ __forceinline__ float max(float v)
     {
         v = wave_max_nan(v);
         if constexpr (G > WAVE) {
@@ -65,7 +65,7 @@ struct Group {
         }
         return v;
     }
-    __device__ float sum(float v)
+    __device__ __forceinline__ float sum(float v)
     {
         v = wave_sum(v);
         if constexpr (G > WAVE) {
@@ -81,7 +81,7 @@ struct Group {
 };
 
 template <class T>
-__device__ inline float logit_at(const T* row, const uint8_t* mask, int j)
+__device__ __forceinline__ float logit_at(const T* row, const uint8_t* mask, int j)
 {
     return (mask && !mask[j]) ? NEG_INF : (float)row[j];
 }
@@ -168,7 +168,7 @@ struct RowLoss {
 
 // (L is a sum of numbers near its own size: in double its difference to
 // old_logp, which is near 0, is exact to the heads' own errors)
-__device__ inline RowLoss row_loss(const LossArgs& a, float adv, float old, double logp, bool possible, float kl, float entropy)
+__device__ __forceinline__ RowLoss row_loss(const LossArgs& a, float adv, float old, double logp, bool possible, float kl, float entropy)
 {
     RowLoss r;
     r.logp = possible ? (float)logp : NEG_INF;
@@ -184,7 +184,7 @@ __device__ inline RowLoss row_loss(const LossArgs& a, float adv, float old, doub
 }
 
 // 1/M, or 0 where there is nothing to take a mean of
-__device__ inline float inverse_rows(const LossArgs& a)
+__device__ __forceinline__ float inverse_rows(const LossArgs& a)
 {
     if (a.denominator > 0.f) return 1.f / a.denominator;
     float m;
@@ -199,7 +199,7 @@ __device__ inline float inverse_rows(const LossArgs& a)
 }
 
 // the blocks' sums to the six numbers of gw_policy_loss's out
-__device__ inline void write_out(const LossArgs& a, const double* s)
+__device__ __forceinline__ void write_out(const LossArgs& a, const double* s)
 {
     const float given = a.denominator > 0.f ? a.denominator : a.denominator_at ? *a.denominator_at : -1.f;
     const double m = given >= 0.f ? (double)given : s[S_COUNT];
@@ -214,7 +214,7 @@ __device__ inline void write_out(const LossArgs& a, const double* s)
 
 // ------------------------------------------------------------ rows out of registers
 template <class T, int CM>
-__device__ inline void store_row(T* row, int width, const float* v)
+__device__ __forceinline__ void store_row(T* row, int width, const float* v)
 {
     constexpr int PER = 16 / sizeof(T);
 #pragma unroll
@@ -231,7 +231,7 @@ __device__ inline void store_row(T* row, int width, const float* v)
 
 // a lane's row into the wave's tile in LDS (rows side by side)
 template <class T, int CM>
-__device__ inline void write_tile(T* row, int width, const float* v)
+__device__ __forceinline__ void write_tile(T* row, int width, const float* v)
 {
     if (sizeof(T) == 2 && (width & 1) == 0) {
 #pragma unroll
@@ -251,7 +251,7 @@ __device__ inline void write_tile(T* row, int width, const float* v)
 
 // the tile to memory, side by side there too
 template <class T>
-__device__ inline void copy_tile(const T* tile, T* to, int n, bool wide, int lane)
+__device__ __forceinline__ void copy_tile(const T* tile, T* to, int n, bool wide, int lane)
 {
     constexpr int PER = 16 / sizeof(T);
     int done = 0;
@@ -264,7 +264,7 @@ __device__ inline void copy_tile(const T* tile, T* to, int n, bool wide, int lan
 
 // a workgroup's sums: to its place among the partial ones, or, where it is the only one, to out
 template <int WAVES>
-__device__ inline void block_sums(const LossArgs& a, double* s)
+__device__ __forceinline__ void block_sums(const LossArgs& a, double* s)
 {
     __shared__ double box[WAVES][N_SUMS];
 #pragma unroll
@@ -286,7 +286,7 @@ __device__ inline void block_sums(const LossArgs& a, double* s)
 // Softmax sums are made in powers of two: the hardware's 2^x, 1/x and log2 x
 // are an ulp off, where float32's own rounding of x (up to 2^-24 |x|) is no less
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-__device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ------------------------------------------------------------- narrow rows
 // A thread a row, the whole row in registers (CM: the width, rounded up).
@@ -312,7 +312,7 @@ struct Tile {
     int64_t base;
     uint32_t l;
     bool there;
-    __device__ Tile(int64_t tile, int64_t rows, int lane) : base(tile * WAVE)
+    __device__ __forceinline__ Tile(int64_t tile, int64_t rows, int lane) : base(tile * WAVE)
     {
         const int64_t left = rows - 1 - base;
         there = lane <= left;
@@ -326,7 +326,7 @@ struct Tile {
 struct Bounds {
     uint64_t starts, ends;
     int32_t width, n, unit, unit_ref;
-    __device__ explicit Bounds(const Small& h)
+    __device__ __forceinline__ explicit Bounds(const Small& h)
         : starts(h.starts), ends(h.ends), width(h.width), n(h.n), unit(h.unit), unit_ref(h.unit_ref)
     {
         asm volatile("" : "+s"(starts), "+s"(ends), "+s"(width), "+s"(n), "+s"(unit), "+s"(unit_ref));
@@ -341,7 +341,7 @@ struct Packed {
     uint32_t w[WORDS];
 
     template <class W>
-    __device__ void load_units(const char* at, int width)
+    __device__ __forceinline__ void load_units(const char* at, int width)
     {
         constexpr int N = sizeof(W) / 4;
 #pragma unroll
@@ -352,7 +352,7 @@ struct Packed {
             }
     }
     // `first`: elements from the uniform `rows` to this lane's row; unit: see Small
-    __device__ void load(const T* rows, uint32_t first, int width, int unit)
+    __device__ __forceinline__ void load(const T* rows, uint32_t first, int width, int unit)
     {
         const char* at = (const char*)rows + first * (uint32_t)sizeof(T);
         if constexpr (WORDS % 4 == 0) {
@@ -371,7 +371,7 @@ struct Packed {
         }
     }
     // -inf behind the row
-    __device__ void get(int width, float* v) const
+    __device__ __forceinline__ void get(int width, float* v) const
     {
 #pragma unroll
         for (int j = 0; j < CM; j++) {
@@ -387,7 +387,7 @@ struct Packed {
 };
 
 template <class T, int CM>
-__device__ inline void load_row(const T* rows, uint32_t first, int width, int unit, float* v)
+__device__ __forceinline__ void load_row(const T* rows, uint32_t first, int width, int unit, float* v)
 {
     Packed<T, CM> p;
     p.load(rows, first, width, unit);
@@ -397,7 +397,7 @@ __device__ inline void load_row(const T* rows, uint32_t first, int width, int un
 // e^x: for 16-bit logits the hardware's 2^x, 2^-20 near for |x| < 16 and far
 // below their own step; for float32 the library's
 template <class T>
-__device__ inline float exp_of(float x)
+__device__ __forceinline__ float exp_of(float x)
 {
     if constexpr (sizeof(T) == 4) return expf(x);
     return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
@@ -405,14 +405,14 @@ __device__ inline float exp_of(float x)
 
 // 1/x and the logarithm of sums of exponentials (from 1 to the width): the
 // hardware's, an ulp or two off
-__device__ inline float rcp_of(float x) { return __builtin_amdgcn_rcpf(x); }
-__device__ inline float log_of(float x) { return __builtin_amdgcn_logf(x) * 0.69314718055994530942f; }
+__device__ __forceinline__ float rcp_of(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ float log_of(float x) { return __builtin_amdgcn_logf(x) * 0.69314718055994530942f; }
 
-__device__ inline bool bit(uint64_t b, int j) { return b >> j & 1; }
+__device__ __forceinline__ bool bit(uint64_t b, int j) { return b >> j & 1; }
 
 // v[j] less its head's maximum (0 where a head has no choice; NaN stays)
 template <int CM>
-__device__ inline void subtract_max(const Bounds& h, float* v)
+__device__ __forceinline__ void subtract_max(const Bounds& h, float* v)
 {
     float m[CM];
 #pragma unroll
@@ -426,7 +426,7 @@ __device__ inline void subtract_max(const Bounds& h, float* v)
 }
 
 // row r uses mask row r % mask_rows
-__device__ inline int64_t mask_row(int64_t mask_rows, int64_t tile_row, uint32_t l)
+__device__ __forceinline__ int64_t mask_row(int64_t mask_rows, int64_t tile_row, uint32_t l)
 {
     const int64_t r = tile_row % mask_rows + l;
     return mask_rows >= WAVE ? (r >= mask_rows ? r - mask_rows : r) : (int64_t)((uint32_t)r % (uint32_t)mask_rows);
@@ -434,7 +434,7 @@ __device__ inline int64_t mask_row(int64_t mask_rows, int64_t tile_row, uint32_t
 
 // masked choices to -inf
 template <int CM>
-__device__ inline void apply_mask(const Packed<uint8_t, CM>& m, float* v)
+__device__ __forceinline__ void apply_mask(const Packed<uint8_t, CM>& m, float* v)
 {
 #pragma unroll
     for (int j = 0; j < CM; j++) v[j] = (m.w[j / 4] >> 8 * (j % 4) & 0xffu) == 0 ? NEG_INF : v[j];
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(256) void sample_narrow_kernel(SampleArgs a, Small 
 constexpr float SPAN = 16.f;
 
 template <int CM>
-__device__ inline bool row_span(const float* v, int width, float& top)
+__device__ __forceinline__ bool row_span(const float* v, int width, float& top)
 {
     float low = -NEG_INF;
     top = NEG_INF;
@@ -526,7 +526,7 @@ __device__ inline bool row_span(const float* v, int width, float& top)
 
 // the same over the choices that exist
 template <int CM>
-__device__ inline bool some_span(const float* v, float top)
+__device__ __forceinline__ bool some_span(const float* v, float top)
 {
     float low = -NEG_INF;
 #pragma unroll
@@ -535,7 +535,7 @@ __device__ inline bool some_span(const float* v, float top)
 }
 
 template <int CM, bool ALL>
-__device__ inline void from_row_top(float top, float* v)
+__device__ __forceinline__ void from_row_top(float top, float* v)
 {
     const float t = ALL || top != NEG_INF ? -top * LOG2E : 0.f;
 #pragma unroll
@@ -546,7 +546,7 @@ __device__ inline void from_row_top(float top, float* v)
 }
 
 template <int CM>
-__device__ inline void from_head_top(const Bounds& h, float* v)
+__device__ __forceinline__ void from_head_top(const Bounds& h, float* v)
 {
     float m[CM];
 #pragma unroll
@@ -591,7 +591,7 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
         int32_t act[4];
         uint8_t valid;
     } next;
-    const auto fetch = [&](int64_t tile) {
+    const auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
         const Tile at_row(tile, a.rows, lane);
         const int64_t base = at_row.base;
         const uint32_t l = at_row.l;
@@ -776,10 +776,10 @@ struct WideRow {
     // Piece k of this lane is piece at(k) of the row.  The row's last piece is
     // read so that it ends with the row: what it shares with the piece before it
     // is marked as no choice, as is a piece behind the row.
-    static __device__ int at(int k) { return L ? k * L + (threadIdx.x & (L ? L - 1 : 0)) : k * (int)blockDim.x + (int)threadIdx.x; }
-    static __device__ int start(int k, int width) { return at(k) * PER < width - PER ? at(k) * PER : width - PER; }
+    static __device__ __forceinline__ int at(int k) { return L ? k * L + (threadIdx.x & (L ? L - 1 : 0)) : k * (int)blockDim.x + (int)threadIdx.x; }
+    static __device__ __forceinline__ int start(int k, int width) { return at(k) * PER < width - PER ? at(k) * PER : width - PER; }
     // pieces that some lane of this wave has
-    static __device__ int pieces(int width)
+    static __device__ __forceinline__ int pieces(int width)
     {
         const int step = L ? L : (int)blockDim.x, first = L ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63);
         int n = 0;
@@ -788,27 +788,27 @@ struct WideRow {
         return n;
     }
 
-    __device__ float get(int k, int e) const
+    __device__ __forceinline__ float get(int k, int e) const
     {
         const uint32_t u = w[k * 4 + e / WORD];
         if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, u);
         else if constexpr (__is_same(T, bf16)) return __builtin_bit_cast(float, e & 1 ? u & 0xffff0000u : u << 16);
         else return (float)__builtin_bit_cast(f16, (uint16_t)(e & 1 ? u >> 16 : u));
     }
-    __device__ void none(int k, int e)
+    __device__ __forceinline__ void none(int k, int e)
     {
         constexpr uint32_t inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, bf16) ? 0xff80u : 0xfc00u;
         uint32_t& u = w[k * 4 + e / WORD];
         if constexpr (sizeof(T) == 4) u = inf;
         else u = e & 1 ? (u & 0xffffu) | inf << 16 : (u & 0xffff0000u) | inf;
     }
-    __device__ void load(const T* row, int width, int n)
+    __device__ __forceinline__ void load(const T* row, int width, int n)
     {
 #pragma unroll
         for (int k = 0; k < V; k++)
             if (k < n) __builtin_memcpy(&w[k * 4], row + start(k, width), 16);   // rows may lie anywhere
     }
-    __device__ void ends(int width, int n)
+    __device__ __forceinline__ void ends(int width, int n)
     {
 #pragma unroll
         for (int k = 0; k < V; k++) {
@@ -819,7 +819,7 @@ struct WideRow {
                     if (e < over) none(k, e);
         }
     }
-    __device__ void mask(const uint8_t* row, int width, int n)
+    __device__ __forceinline__ void mask(const uint8_t* row, int width, int n)
     {
 #pragma unroll
         for (int k = 0; k < V; k++) {
@@ -832,7 +832,7 @@ struct WideRow {
         }
     }
     // choices that the other row has not are none here
-    __device__ void only(const WideRow& o, int n)
+    __device__ __forceinline__ void only(const WideRow& o, int n)
     {
 #pragma unroll
         for (int k = 0; k < V; k++)
@@ -842,7 +842,7 @@ struct WideRow {
                     if (o.get(k, e) == NEG_INF) none(k, e);
     }
     // the largest logit, and the smallest (-inf: some choice does not exist)
-    __device__ void range(float& hi, float& lo, int n) const
+    __device__ __forceinline__ void range(float& hi, float& lo, int n) const
     {
         hi = NEG_INF;
         lo = -NEG_INF;
@@ -859,7 +859,7 @@ struct WideRow {
     // size: one fma; its rounding of `top` is common to all choices and to
     // their sum, so it cancels
     template <bool PLAIN>
-    __device__ float less(int k, int e, float top) const
+    __device__ __forceinline__ float less(int k, int e, float top) const
     {
         const float z = get(k, e);
         if constexpr (PLAIN) return fmaf(z, LOG2E, -top * LOG2E);
@@ -868,7 +868,7 @@ struct WideRow {
         return z == NEG_INF ? NO_CHOICE : x < -1e30f ? -1e30f : x;
     }
     // what was made of the row before is not to be kept beside it: it is made again
-    __device__ void forget()
+    __device__ __forceinline__ void forget()
     {
 #pragma unroll
         for (int i = 0; i < V * 4; i++) asm volatile("" : "+v"(w[i]));
@@ -877,7 +877,7 @@ struct WideRow {
 
 // sums or maxima of M values over a row's lanes
 template <int L, int M, class Op>
-__device__ inline void over_group(float* v, float (*box)[16], Op op)
+__device__ __forceinline__ void over_group(float* v, float (*box)[16], Op op)
 {
 #pragma unroll
     for (int o = (L ? L : WAVE) / 2; o > 0; o >>= 1)
@@ -906,8 +906,8 @@ struct OneHead { int32_t width, low, slot, act_dim; };
 template <int L>
 struct Rows {
     static constexpr int PER_BLOCK = L ? 256 / (L ? L : 1) : 1;
-    static __device__ int64_t first() { return L ? (int64_t)blockIdx.x * PER_BLOCK + threadIdx.x / (L ? L : 1) : blockIdx.x; }
-    static __device__ bool leader() { return L ? (threadIdx.x & (L ? L - 1 : 0)) == 0 : threadIdx.x == 0; }
+    static __device__ __forceinline__ int64_t first() { return L ? (int64_t)blockIdx.x * PER_BLOCK + threadIdx.x / (L ? L : 1) : blockIdx.x; }
+    static __device__ __forceinline__ bool leader() { return L ? (threadIdx.x & (L ? L - 1 : 0)) == 0 : threadIdx.x == 0; }
 };
 
 template <class T, int V, int L>
@@ -953,7 +953,7 @@ __global__ __launch_bounds__(L ? 256 : 1024) void sample_wide_kernel(SampleArgs 
         over_group<L, 1>(m, box, [](float p, float q) { return fmaxf(p, q); });
         const float top = m[0] == NEG_INF ? 0.f : m[0];
         float q[2] = {0.f, 0.f};
-        const auto sum = [&](auto plain) {
+        const auto sum = [&](auto plain) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < V; k++) {
                 if (k >= pieces) continue;
@@ -1035,7 +1035,7 @@ __global__ __launch_bounds__(L ? 256 : 1024) void loss_wide_kernel(LossArgs a, O
         const float top = m[0] == NEG_INF ? 0.f : m[0], top_r = m[1] == NEG_INF ? 0.f : m[1];
         // (by waves: most rows are plain but for the pieces behind their ends)
         const bool plain_wave = __all(low > -1e30f && low_r > -1e30f && fabsf(top) < 1e30f && fabsf(top_r) < 1e30f);
-        const auto sum = [&](auto plain) {
+        const auto sum = [&](auto plain) __attribute__((always_inline)) {
             constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
             for (int k = 0; k < V; k++) {
@@ -1080,7 +1080,7 @@ __global__ __launch_bounds__(L ? 256 : 1024) void loss_wide_kernel(LossArgs a, O
             // (log p + H = x - T/S)
             const float pull = got.pull * scale, eta = a.entropy * scale * LN2, beta = a.kl * scale;
             const float a1 = eta * inv, a0 = inv * ((some_ref ? beta : 0.f) - pull - eta * ts), b = -beta * inv_r;
-            const auto walk = [&](auto plain) {
+            const auto walk = [&](auto plain) __attribute__((always_inline)) {
                 constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
                 for (int k = 0; k < V; k++) {

@@ -34,15 +34,15 @@ struct Map { float a, b; };
 
 // A map drops the state only where a gate is 0.  The product of others may
 // underflow: then the smallest number keeps an infinite state infinite.
-__device__ inline float keep(float a, bool zero) { return zero ? 0.f : (a == 0.f ? 1.4e-45f : a); }
+__device__ __forceinline__ float keep(float a, bool zero) { return zero ? 0.f : (a == 0.f ? 1.4e-45f : a); }
 
 // a h + b, where a = 0 drops any state (0 * inf would be NaN)
-__device__ inline float advance(float a, float h, float b) { return fmaf(a, a == 0.f ? 0.f : h, b); }
+__device__ __forceinline__ float advance(float a, float h, float b) { return fmaf(a, a == 0.f ? 0.f : h, b); }
 
 // the same for a segment's map, whose product of gates may have overflowed
-__device__ inline float apply(Map m, float h) { return m.a == 0.f || h == 0.f ? m.b : fmaf(m.a, h, m.b); }
+__device__ __forceinline__ float apply(Map m, float h) { return m.a == 0.f || h == 0.f ? m.b : fmaf(m.a, h, m.b); }
 
-__device__ inline Map compose(Map first, Map then)
+__device__ __forceinline__ Map compose(Map first, Map then)
 {
     return Map{keep(first.a * then.a, first.a == 0.f || then.a == 0.f), apply(then, first.b)};
 }
@@ -53,7 +53,7 @@ struct Chunks { int32_t count; int64_t steps; float2* maps; };
 // The state that reaches wave w's segment, from the one that reaches the
 // tile (`in`, which becomes the one behind the tile) and the waves' maps.
 template <int NW>
-__device__ inline float join(float2 (*box)[WAVE], int w, int lane, Map m, float& in)
+__device__ __forceinline__ float join(float2 (*box)[WAVE], int w, int lane, Map m, float& in)
 {
     box[w][lane] = make_float2(m.a, m.b);
     __syncthreads();
@@ -71,7 +71,7 @@ __device__ inline float join(float2 (*box)[WAVE], int w, int lane, Map m, float&
 // The state that reaches a chunk: `state` through the maps of the chunks
 // before it, shared out to the NW waves.
 template <int NW>
-__device__ inline float reach_chunk(float2 (*box)[WAVE], const Chunks& s, int64_t n, int64_t c, int w, int lane,
+__device__ __forceinline__ float reach_chunk(float2 (*box)[WAVE], const Chunks& s, int64_t n, int64_t c, int w, int lane,
                                     float state)
 {
     const int chunk = blockIdx.y;
@@ -99,11 +99,11 @@ struct Place {
     int w, lane;
     uint32_t l;
     bool on;
-    __device__ int64_t c() const { return c0 + l; }
+    __device__ __forceinline__ int64_t c() const { return c0 + l; }
 };
 
 template <int NW, int CW>
-__device__ inline Place place(int64_t n)
+__device__ __forceinline__ Place place(int64_t n)
 {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     Place p;
@@ -120,7 +120,7 @@ __device__ inline Place place(int64_t n)
 // a uniform place, per lane a small offset
 struct Shared {
     uint32_t first, l;
-    __device__ Shared(uint32_t span, const Place& p)
+    __device__ __forceinline__ Shared(uint32_t span, const Place& p)
     {
         // (fewer than 2^31 channels)
         first = (uint32_t)p.c0 / span;
@@ -129,13 +129,13 @@ struct Shared {
 };
 
 // step i of the recurrence's own order is step at(i) of the slabs
-__device__ inline int64_t step_at(const RecurArgs& a, int64_t i) { return a.reverse ? a.T - 1 - i : i; }
+__device__ __forceinline__ int64_t step_at(const RecurArgs& a, int64_t i) { return a.reverse ? a.T - 1 - i : i; }
 
 // SEG rows of `stride` values from step i0 on, one value a lane: f(k, value).
 // Whole segments are one run of loads; in the last one the steps that are
 // there are a uniform branch each.
 template <class V, class F>
-__device__ inline void load_rows(const RecurArgs& a, const V* slab, int64_t stride, int64_t i0, int64_t first,
+__device__ __forceinline__ void load_rows(const RecurArgs& a, const V* slab, int64_t stride, int64_t i0, int64_t first,
                                  uint32_t l, F f)
 {
     const V* row = slab + step_at(a, i0) * stride + first;
@@ -157,7 +157,7 @@ __device__ inline void load_rows(const RecurArgs& a, const V* slab, int64_t stri
 // The gates of SEG steps from i0 (0 where cut; 1 behind the last step), and
 // cuts as bits
 template <class TG>
-__device__ inline uint32_t load_gates(const RecurArgs& a, int64_t i0, const Shared& g, const Shared& c, float* gate)
+__device__ __forceinline__ uint32_t load_gates(const RecurArgs& a, int64_t i0, const Shared& g, const Shared& c, float* gate)
 {
     uint32_t bits = 0;
     const int m = i0 + SEG <= a.T ? SEG : (int)(a.T - i0);
@@ -174,7 +174,7 @@ __device__ inline uint32_t load_gates(const RecurArgs& a, int64_t i0, const Shar
 
 // SEG steps of a slab like x; 0 behind the last step
 template <class T>
-__device__ inline void load_values(const RecurArgs& a, const void* slab, int64_t i0, const Place& p, float* v)
+__device__ __forceinline__ void load_values(const RecurArgs& a, const void* slab, int64_t i0, const Place& p, float* v)
 {
 #pragma unroll
     for (int k = 0; k < SEG; k++) v[k] = 0.f;
@@ -184,7 +184,7 @@ __device__ inline void load_values(const RecurArgs& a, const void* slab, int64_t
 // The map of a segment: forwards h -> gate h + x, or (BACK) from the last step
 // to the first into -> gate (into + dh)
 template <bool BACK>
-__device__ inline Map segment_map(const float* gate, const float* v)
+__device__ __forceinline__ Map segment_map(const float* gate, const float* v)
 {
     Map m{1.f, 0.f};
     bool zero = false;
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(64 * NW * CW) void recur_kernel(RecurArgs a, Chunks
     const Shared g(a.gate_span, p), c(a.cut_span, p);
     const int64_t from = blockIdx.y * s.steps, to = from + s.steps < a.T ? from + s.steps : a.T;
     float gate[SEG], x[SEG];
-    const auto fetch = [&](int64_t i0) {
+    const auto fetch = [&](int64_t i0) __attribute__((always_inline)) {
         if (i0 >= a.T) return;
         load_gates<TG>(a, i0, g, c, gate);
         load_values<T>(a, a.x, i0, p, x);
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(64 * NW * CW) void recur_kernel(RecurArgs a, Chunks
 // few whole gates and parts of two.  d crosses LDS; then every lane adds the
 // channels of (step, gate) pairs, in their order.
 template <class TG>
-__device__ inline void gate_sums(const RecurArgs& a, float (*tile)[WAVE + 1], int64_t i0, const Place& p, const float* d)
+__device__ __forceinline__ void gate_sums(const RecurArgs& a, float (*tile)[WAVE + 1], int64_t i0, const Place& p, const float* d)
 {
 #pragma unroll
     for (int k = 0; k < SEG; k++) tile[k][p.lane] = p.on ? d[k] : 0.f;
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(64 * NW * CW) void recur_backward_kernel(RecurArgs 
     const int64_t from = blockIdx.y * s.steps, to = from + s.steps < segs * SEG ? from + s.steps : segs * SEG;
     float gate[SEG], before[SEG], dh[SEG];
     uint32_t cut = 0;
-    const auto fetch = [&](int64_t i0) {
+    const auto fetch = [&](int64_t i0) __attribute__((always_inline)) {
         if (i0 < 0) return;
         float x[SEG];
         cut = load_gates<TG>(a, i0, g, c, gate);
@@ -410,7 +410,7 @@ struct AdvArgs {
 // One segment of a lane's steps: for each step the map carry -> gate carry +
 // delta, the value (0 where the lane did not act) and whether it acted.
 template <class TR, class TV>
-__device__ inline uint32_t load_steps(const AdvArgs& a, int64_t n, int64_t i0, const Place& p, const Shared& env,
+__device__ __forceinline__ uint32_t load_steps(const AdvArgs& a, int64_t n, int64_t i0, const Place& p, const Shared& env,
                                       bool acts, float* gate, float* delta, float* value)
 {
     uint8_t done[SEG + 1], mark[SEG + 1];       // [k]: of the step before step k

@@ -767,3 +767,16 @@ def test_autograd_refuses_changed_inputs():
     args[1].add_(1)
     with pytest.raises(RuntimeError, match='inplace'):
         r.loss.backward()
+
+
+def test_kernels_call_nothing():
+    """Every helper is inlined (a called function would need a stack of its
+    own) and no kernel spills more than a few scalars."""
+    pytest.importorskip('msgpack')
+    from tests.test_kernel_resources import kernel_metadata
+    _native.build_learn()
+    md = kernel_metadata(_native.LIB_LEARN)
+    assert len(md) > 50
+    bad = {k: v['.private_segment_fixed_size'] for k, v in md.items()
+           if v['.private_segment_fixed_size'] > 64 or v.get('.uses_dynamic_stack')}
+    assert not bad, bad
