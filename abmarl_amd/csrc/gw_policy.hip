@@ -1269,7 +1269,7 @@ __global__ __launch_bounds__(2 * N_SUMS * WAVE) void finish_kernel(LossArgs a, i
 }
 
 constexpr int MAX_BLOCKS = 8192;
-constexpr int64_t NARROW_BLOCKS = 2048;         // 256 CUs, 8 workgroups of 4 waves each
+constexpr int64_t NARROW_BLOCKS = 1024;         // 256 CUs, 8 workgroups of 4 waves each
 
 // the host's heads, checked, as the kernels take them
 gw_status take_heads(const gw_policy_heads* p, Heads* h)

@@ -10,7 +10,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from abmarl_amd import _abi, _native
+from abmarl_amd import _abi, _native, learning
 
 
 def _ptr(t):
@@ -328,6 +328,82 @@ class GridWorldEngine:
                                                    int(env_offset) & 0xFFFFFFFF, _ptr(out),
                                                    _stream()), 'gw_random_actions')
         return out
+
+    # ------------------------------------------------- policies (learning.py)
+    def policy_heads(self):
+        """The softmax heads over this engine's action rows, and what each lane
+        may choose: (learning.PolicyHeads, choice mask uint8 [A][n_choices],
+        acts uint8 [A], the lanes that act at all).  Moves are 2 heads over
+        -r..r (Pacman: one over its 5 cross moves), the attack one head over
+        0..simultaneous_attacks, or one for each cell of the attack window; a
+        lane that cannot move or attack has the one choice 0 there, as
+        random_actions gives it."""
+        if getattr(self, '_heads', None) is None:
+            specs = [self.cc.specs[i] for i in self.lane_entities]
+            cross = [s.kind & _abi.GW_K_MOVING != 0 for s in specs]
+            move = [s.move_range if m else 0 for s, m in zip(specs, cross)]
+            simul = [s.simultaneous_attacks if s.kind & _abi.GW_K_ATTACKING else 0 for s in specs]
+            if self.pacman:
+                heads = learning.PolicyHeads([5], slots=[0], act_dim=self.act_dim)
+                rows = [[1] + [int(m)] * 4 for m in cross]
+            else:
+                r, k, cells = max(move), max(simul), self.act_dim - 2
+                heads = learning.PolicyHeads([2 * r + 1] * 2 + [k + 1] * cells, low=[-r] * 2 + [0] * cells)
+                rows = []
+                for s, m, n in zip(specs, move, simul):
+                    own = cells if cells == 1 else (2 * s.attack_range + 1) ** 2
+                    rows.append([int(abs(v) <= m) for v in range(-r, r + 1)] * 2 +
+                                [int(v == 0 or (q < own and v <= n)) for q in range(cells) for v in range(k + 1)])
+            acts = [int(s.kind & _abi.GW_K_ACTING != 0) for s in specs]
+            self._heads = (heads, torch.tensor(rows, dtype=torch.uint8, device=self.device),
+                           torch.tensor(acts, dtype=torch.uint8, device=self.device))
+        return self._heads
+
+    def sample_actions(self, logits, noise=None, out=None):
+        """Action rows drawn from a policy's logits [..., A, n_choices]
+        (learning.sample_actions with policy_heads): for logits [E, A, n] they
+        go into self.actions, which step() takes, unless `out` is given."""
+        heads, mask, _ = self.policy_heads()
+        if out is None and logits.shape[:-1] == self.actions.shape[:-1]:
+            out = self.actions
+        return learning.sample_actions(logits, heads, noise, mask, out=out)
+
+    def fragment_start(self):
+        """What advantages() needs of the envs before a fragment: their step
+        counters, live lanes and '__all__' (a copy)."""
+        E, A, dev = self.E, self.A, self.device
+        steps = torch.empty((E,), dtype=torch.int32, device=dev)
+        flags = torch.empty((E, A), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            _native.check(self.L.gw_get_state(self.h, None, None, _ptr(flags), None, None, _ptr(steps), _stream()),
+                          'gw_get_state')
+        return dict(steps=steps, live=(flags & _abi.FLAG_LIVE != 0).to(torch.uint8), all_done=self.all_done.clone())
+
+    def advantages(self, out, value, start, gamma=0.99, lam=0.95, horizon=0, autoreset='next_step'):
+        """learning.advantages of a fragment: `out` its slabs (rollout(), or
+        step_autoreset[_next] outputs stacked), value [K + 1, E, A] of the
+        observations before each step and after the last, start
+        fragment_start() before it; horizon and autoreset the fragment's.
+        Envs whose error flags are set are left out (valid 0): zero
+        engine.err before the fragment."""
+        if 'returned' in out:
+            raise ValueError("turn-based slabs: a lane's steps are turns apart, advantages are not defined over them")
+        K = int(value.shape[0]) - 1
+        marks = learning.fragment_marks(out['all_done'][:K], start['steps'], horizon, autoreset, start['all_done'],
+                                        self.err)
+        return learning.advantages(out['reward'][:K], value, out['done'][:K], marks, start['live'], gamma, lam,
+                                   acts=self.policy_heads()[2])
+
+    def policy_loss(self, logits, actions, advantage, old_logp, **kw):
+        """learning.policy_loss with this engine's heads and lane masks
+        (logits [..., A, n_choices], actions [..., A, act_dim])."""
+        heads, mask, _ = self.policy_heads()
+        return learning.policy_loss(logits, actions, advantage, old_logp, heads, choice_mask=mask, **kw)
+
+    def policy_loss_grad(self, logits, actions, advantage, old_logp, **kw):
+        """learning.policy_loss_grad with this engine's heads and lane masks."""
+        heads, mask, _ = self.policy_heads()
+        return learning.policy_loss_grad(logits, actions, advantage, old_logp, heads, choice_mask=mask, **kw)
 
     AUTORESET_MODES = {'none': 0, 'same_step': 1, 'next_step': 2}
 
