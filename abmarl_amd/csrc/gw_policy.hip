@@ -86,8 +86,12 @@ __device__ __forceinline__ float logit_at(const T* row, const uint8_t* mask, int
     return (mask && !mask[j]) ? NEG_INF : (float)row[j];
 }
 
-// One row by one workgroup of G threads, the choices of a head strided over
-// them.  Right for every layout: any number of heads, any width.
+// Rows that neither fit a thread nor are one head: a row by a workgroup of G
+// threads.  Heads of up to LANE_HEAD choices are walked by one lane each (the
+// cells of an attack window are dozens of heads of a few choices), larger ones
+// by the whole group, their choices strided over it.  Right for every layout.
+constexpr int LANE_HEAD = 16;
+
 template <class T, int G>
 __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
 {
@@ -101,15 +105,44 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
         const float* noise = a.noise ? a.noise + row * h.width : nullptr;
         const uint8_t* mask = a.mask ? a.mask + (row % a.mask_rows) * h.width : nullptr;
         int32_t* act = a.actions + row * h.act_dim;
-        for (int c = tid; c < h.act_dim; c += G) {
-            bool owned = false;
-            for (int d = 0; d < h.n; d++) owned |= h.slot[d] == c;
-            if (!owned) act[c] = 0;
+        if (h.n < h.act_dim)
+            for (int c = tid; c < h.act_dim; c += G) {
+                bool owned = false;
+                for (int d = 0; d < h.n; d++) owned |= h.slot[d] == c;
+                if (!owned) act[c] = 0;
+            }
+        float logp = 0.f, entropy = 0.f;                 // of this lane's heads; the group's in lane 0
+        for (int d = tid; d < h.n; d += G) {
+            const int lo = h.off[d], hi = h.off[d + 1];
+            if (hi - lo > LANE_HEAD) continue;
+            float m = NEG_INF, bs = NEG_INF, at = 0.f, s = 0.f, t = 0.f;
+            int bi = -1;
+            for (int j = lo; j < hi; j++) {
+                const float v = logit_at(z, mask, j);
+                if (v == NEG_INF) continue;
+                m = max_nan(m, v);
+                const float sc = noise ? v + noise[j] : v;
+                if (sc > bs || (bi < 0 && sc == bs)) { bs = sc; bi = j; at = v; }
+            }
+            if (m != NEG_INF) {
+                for (int j = lo; j < hi; j++) {
+                    const float v = logit_at(z, mask, j);
+                    if (v == NEG_INF) continue;
+                    const float e = expf(v - m);
+                    s += e;
+                    t += e * (v - m);
+                }
+                const float log_s = logf(s);
+                logp += (at - m) - log_s;
+                entropy += log_s - t / s;
+            }
+            act[h.slot[d]] = h.low[d] + (bi < 0 ? 0 : bi - lo);
         }
-        double logp = 0.;
-        float entropy = 0.f;
+        double row_logp = 0.;
+        float row_entropy = 0.f;
         for (int d = 0; d < h.n; d++) {
             const int lo = h.off[d], hi = h.off[d + 1];
+            if (hi - lo <= LANE_HEAD) continue;
             float m = NEG_INF, bs = NEG_INF;
             int bi = INT32_MAX;
             for (int j = lo + tid; j < hi; j += G) {
@@ -149,13 +182,15 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
             s = grp.sum(s);
             t = grp.sum(t);
             const float log_s = logf(s);
-            logp += (double)(logit_at(z, mask, bi) - m) - (double)log_s;
-            entropy += log_s - t / s;
+            row_logp += (double)(logit_at(z, mask, bi) - m) - (double)log_s;
+            row_entropy += log_s - t / s;
             if (tid == 0) act[h.slot[d]] = h.low[d] + (bi - lo);
         }
+        logp = grp.sum(logp);
+        entropy = grp.sum(entropy);
         if (tid == 0) {
-            if (a.logp) a.logp[row] = (float)logp;
-            if (a.entropy) a.entropy[row] = entropy;
+            if (a.logp) a.logp[row] = (float)(row_logp + (double)logp);
+            if (a.entropy) a.entropy[row] = row_entropy + entropy;
         }
     }
 }
@@ -1144,11 +1179,53 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
         const T* zr = a.ref ? (const T*)a.ref + row * a.ld_ref : nullptr;
         const uint8_t* mask = a.mask ? a.mask + (row % a.mask_rows) * h.width : nullptr;
         const int32_t* act = a.actions + row * h.act_dim;
+        // this lane's heads: their parts of L, KL, H, and how many actions were not possible
+        float mine[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int d = tid; d < h.n; d += G) {
+            const int lo = h.off[d], hi = h.off[d + 1];
+            if (hi - lo > LANE_HEAD) continue;
+            float m = NEG_INF, mr = NEG_INF, s = 0.f, t = 0.f, sr = 0.f, u = 0.f;
+            for (int j = lo; j < hi; j++) {
+                const float v = logit_at(z, mask, j);
+                if (v == NEG_INF) continue;
+                m = max_nan(m, v);
+                if (zr) mr = max_nan(mr, (float)zr[j]);
+            }
+            float log_s = 0.f, inv = 0.f, ent = 0.f, inv_r = 0.f;
+            if (m != NEG_INF) {
+                for (int j = lo; j < hi; j++) {
+                    const float v = logit_at(z, mask, j);
+                    if (v == NEG_INF) continue;
+                    const float e = expf(v - m);
+                    s += e;
+                    t += e * (v - m);
+                    if (zr && (float)zr[j] != NEG_INF) {
+                        const float w = (float)zr[j] - mr, er = expf(w);
+                        sr += er;
+                        u += er * (w - (v - m));
+                    }
+                }
+                log_s = logf(s);
+                inv = 1.f / s;
+                ent = log_s - t * inv;
+                mine[2] += ent;
+                if (zr && mr != NEG_INF) {
+                    inv_r = 1.f / sr;
+                    mine[1] += u * inv_r + logf(s * inv_r);
+                }
+                const int c = act[h.slot[d]] - h.low[d];
+                const float v = c >= 0 && c < hi - lo ? logit_at(z, mask, lo + c) : NEG_INF;
+                if (v == NEG_INF) mine[3] += 1.f;
+                else mine[0] += (v - m) - log_s;
+            }
+            hm[d] = m; hls[d] = log_s; hinv[d] = inv; hh[d] = ent; hrm[d] = mr; hrinv[d] = inv_r;
+        }
         float kl = 0.f, entropy = 0.f;
         double logp = 0.;
         bool possible = true;
         for (int d = 0; d < h.n; d++) {
             const int lo = h.off[d], hi = h.off[d + 1];
+            if (hi - lo <= LANE_HEAD) continue;
             float m = NEG_INF, mr = NEG_INF;
             for (int j = lo + tid; j < hi; j += G) {
                 const float v = logit_at(z, mask, j);
@@ -1194,27 +1271,42 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                 hm[d] = m; hls[d] = log_s; hinv[d] = inv; hh[d] = ent; hrm[d] = mr; hrinv[d] = inv_r;
             }
         }
-        const RowLoss r = row_loss(a, a.advantage[row], a.old_logp[row], logp, possible, kl, entropy);
+#pragma unroll
+        for (int k = 0; k < 4; k++) mine[k] = grp.sum(mine[k]);
+        const RowLoss r = row_loss(a, a.advantage[row], a.old_logp[row], logp + (double)mine[0], possible && mine[3] == 0.f,
+                                   kl + mine[1], entropy + mine[2]);
         if (tid == 0) {
             if (a.logp) a.logp[row] = r.logp;
             sums[S_PG] += r.pg; sums[S_KL] += r.kl; sums[S_H] += r.entropy;
             sums[S_CLIP] += r.clipped ? 1. : 0.; sums[S_COUNT] += 1.;
         }
-        if (!g) continue;
+        if (!g) {
+            __syncthreads();                             // the next row's heads go where this one's are
+            continue;
+        }
         __syncthreads();
-        for (int d = 0; d < h.n; d++) {
-            const int lo = h.off[d], hi = h.off[d + 1], c = act[h.slot[d]] - h.low[d];
-            for (int j = lo + tid; j < hi; j += G) {
-                const float v = logit_at(z, mask, j);
-                float gj = 0.f;
-                if (v != NEG_INF) {
-                    const float x = v - hm[d], p = expf(x) * hinv[d];
-                    // d(-surrogate) pull (1[chosen] - p), KL p - q, entropy p (log p + H)
-                    gj = r.pull * ((j - lo == c ? 1.f : 0.f) - p) + a.entropy * p * (x - hls[d] + hh[d]);
-                    if (hrinv[d] != 0.f) gj += a.kl * (p - expf((float)zr[j] - hrm[d]) * hrinv[d]);
-                }
-                g[j] = (T)(gj * step);
+        const auto one = [&](int d, int j, int c) __attribute__((always_inline)) {
+            const float v = logit_at(z, mask, j);
+            float gj = 0.f;
+            if (v != NEG_INF) {
+                const float x = v - hm[d], p = expf(x) * hinv[d];
+                // d(-surrogate) pull (1[chosen] - p), KL p - q, entropy p (log p + H)
+                gj = r.pull * ((j - h.off[d] == c ? 1.f : 0.f) - p) + a.entropy * p * (x - hls[d] + hh[d]);
+                if (hrinv[d] != 0.f) gj += a.kl * (p - expf((float)zr[j] - hrm[d]) * hrinv[d]);
             }
+            g[j] = (T)(gj * step);
+        };
+        for (int d = tid; d < h.n; d += G) {
+            const int lo = h.off[d], hi = h.off[d + 1];
+            if (hi - lo > LANE_HEAD) continue;
+            const int c = act[h.slot[d]] - h.low[d];
+            for (int j = lo; j < hi; j++) one(d, j, c);
+        }
+        for (int d = 0; d < h.n; d++) {
+            const int lo = h.off[d], hi = h.off[d + 1];
+            if (hi - lo <= LANE_HEAD) continue;
+            const int c = act[h.slot[d]] - h.low[d];
+            for (int j = lo + tid; j < hi; j += G) one(d, j, c);
         }
         __syncthreads();
     }
@@ -1269,7 +1361,7 @@ __global__ __launch_bounds__(2 * N_SUMS * WAVE) void finish_kernel(LossArgs a, i
 }
 
 constexpr int MAX_BLOCKS = 8192;
-constexpr int64_t NARROW_BLOCKS = 1024;         // 256 CUs, 8 workgroups of 4 waves each
+constexpr int64_t NARROW_BLOCKS = 1024;         // 256 CUs, 4 workgroups of 4 waves each
 
 // the host's heads, checked, as the kernels take them
 gw_status take_heads(const gw_policy_heads* p, Heads* h)
@@ -1397,7 +1489,8 @@ void launch_sample(const SampleArgs& a, const Heads& h, hipStream_t st)
         return;
     }
     const dim3 grid((unsigned)blocks_for(a.rows));
-    if (h.width >= 1024) hipLaunchKernelGGL((sample_rows_kernel<T, 256>), grid, dim3(256), 0, st, a, h);
+    if (h.width >= 8192) hipLaunchKernelGGL((sample_rows_kernel<T, 1024>), grid, dim3(1024), 0, st, a, h);
+    else if (h.width >= 1024) hipLaunchKernelGGL((sample_rows_kernel<T, 256>), grid, dim3(256), 0, st, a, h);
     else hipLaunchKernelGGL((sample_rows_kernel<T, 64>), grid, dim3(64), 0, st, a, h);
 }
 
@@ -1469,7 +1562,8 @@ unsigned launch_loss(const LossArgs& a, const Heads& h, hipStream_t st)
         return blocks;
     }
     const unsigned blocks = (unsigned)blocks_for(a.rows);
-    if (h.width >= 1024) hipLaunchKernelGGL((loss_rows_kernel<T, 256>), dim3(blocks), dim3(256), 0, st, a, h);
+    if (h.width >= 8192) hipLaunchKernelGGL((loss_rows_kernel<T, 1024>), dim3(blocks), dim3(1024), 0, st, a, h);
+    else if (h.width >= 1024) hipLaunchKernelGGL((loss_rows_kernel<T, 256>), dim3(blocks), dim3(256), 0, st, a, h);
     else hipLaunchKernelGGL((loss_rows_kernel<T, 64>), dim3(blocks), dim3(64), 0, st, a, h);
     return blocks;
 }

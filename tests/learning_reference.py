@@ -46,7 +46,7 @@ def sample(logits, heads, noise=None, mask=None):
             if t.any():
                 score = z32[r, s] + noise[r, s] if noise is not None else z32[r, s].clone()   # float32, as defined
                 score[~t] = -math.inf
-                choice = min(i for i in range(len(t)) if t[i] and score[i] == score[t].max())
+                choice = int(torch.nonzero(t & (score == score[t].max()))[0])
                 lp, p, h = softmax_row(z[r, s], t)
                 logp[r] += lp[choice]
                 entropy[r] += h

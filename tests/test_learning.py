@@ -209,9 +209,10 @@ LAYOUTS = {
     'odd': PolicyHeads([7, 1, 31], low=[-3, 5, 0], slots=[3, 0, 1], act_dim=6),
     'w63': PolicyHeads([63]), 'w64': PolicyHeads([64]), 'w65': PolicyHeads([65]), 'w200': PolicyHeads([129, 71]),
     'w513': PolicyHeads([513]), 'w1031': PolicyHeads([1031]), 'w4100': PolicyHeads([4100]),
-    'many': PolicyHeads([15, 15] + [2] * 225), 'mixed': PolicyHeads([3, 1500, 2, 700]),
+    'w40003': PolicyHeads([40003]), 'two_wide': PolicyHeads([5000, 3, 5000]),
+    'many': PolicyHeads([15, 15] + [2] * 225), 'cells': PolicyHeads([17, 17] + [4] * 49), 'mixed': PolicyHeads([3, 1500, 2, 700]),
 }
-ROWS = {'w513': 9, 'w1031': 5, 'w4100': 3, 'many': 7, 'mixed': 4, 'w200': 13}
+ROWS = {'w513': 9, 'w1031': 5, 'w4100': 3, 'many': 7, 'mixed': 4, 'w200': 13, 'w40003': 2, 'two_wide': 2, 'cells': 11}
 
 
 def inputs(name, dtype, seed, masked, lanes=None):
