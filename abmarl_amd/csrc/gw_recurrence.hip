@@ -359,6 +359,117 @@ __global__ __launch_bounds__(64 * NW * CW) void recur_backward_kernel(RecurArgs 
     if (a.dstate && p.on && p.w == 0 && to == segs * SEG) a.dstate[p.c()] = in;
 }
 
+// ------------------------------------------------------------- pairs of channels
+// 16-bit slabs of many channels: a lane takes two neighbouring channels (one
+// 4-byte load a step), kept as they lie in memory until their step.  The
+// arguments count pairs: n, gate_span and cut_span are halved, a pair shares its
+// cut and, where gates are shared (SHARED), its gate.
+template <class T>
+struct Two { T a, b; };
+
+template <class T, class TG, bool SHARED>
+struct PairSegment {
+    Two<T> v[SEG];
+    TG gate[SHARED ? SEG : 1];
+    Two<TG> gates[SHARED ? 1 : SEG];
+    uint32_t cut = 0;
+
+    __device__ __forceinline__ void load_gates(const RecurArgs& a, int64_t i0, const Place& p, const Shared& g, const Shared& c)
+    {
+        cut = 0;
+        if constexpr (SHARED) {
+            if (a.gate) load_rows(a, (const TG*)a.gate, a.gates, i0, g.first, g.l, [&](int k, TG x) { gate[k] = x; });
+        } else {
+            load_rows(a, (const Two<TG>*)a.gate, a.n, i0, p.c0, p.l, [&](int k, Two<TG> x) { gates[k] = x; });
+        }
+        if (a.cut) load_rows(a, a.cut, a.cuts, i0, c.first, c.l, [&](int k, uint8_t x) { cut |= (x ? 1u : 0u) << k; });
+    }
+    __device__ __forceinline__ float2 at(const RecurArgs& a, int k) const
+    {
+        float2 r;
+        if constexpr (SHARED) r.x = r.y = a.gate ? (float)gate[k] : a.gate_value;
+        else r = make_float2((float)gates[k].a, (float)gates[k].b);
+        return cut >> k & 1 ? make_float2(0.f, 0.f) : r;
+    }
+};
+
+template <class T, class TG, bool SHARED>
+__global__ __launch_bounds__(256) void recur_pair_kernel(RecurArgs a)
+{
+    const Place p = place<1, 4>(a.n);
+    if (p.c0 >= a.n) return;
+    const Shared g(a.gate_span, p), c(a.cut_span, p);
+    const int64_t next = a.reverse ? -a.n : a.n;
+    float2 h = a.state ? ((const float2*)a.state)[p.c()] : make_float2(0.f, 0.f);
+    for (int64_t i0 = 0; i0 < a.T; i0 += SEG) {
+        PairSegment<T, TG, SHARED> s;
+        s.load_gates(a, i0, p, g, c);
+        load_rows(a, (const Two<T>*)a.x, a.n, i0, p.c0, p.l, [&](int k, Two<T> x) { s.v[k] = x; });
+        if (p.on && a.carry) ((float2*)a.carry)[i0 / SEG * a.n + p.c()] = h;
+        const int m = i0 + SEG <= a.T ? SEG : (int)(a.T - i0);
+        Two<T>* row = (Two<T>*)a.h + step_at(a, i0) * a.n + p.c0;
+#pragma unroll
+        for (int k = 0; k < SEG; k++, row += next) {
+            if (k >= m) continue;
+            const float2 q = s.at(a, k);
+            h.x = advance(q.x, h.x, (float)s.v[k].a);
+            h.y = advance(q.y, h.y, (float)s.v[k].b);
+            if (p.on) row[p.l] = Two<T>{(T)h.x, (T)h.y};
+        }
+    }
+    if (a.last && p.on) ((float2*)a.last)[p.c()] = h;
+}
+
+template <class T, class TG, bool SHARED>
+__global__ __launch_bounds__(256) void recur_backward_pair_kernel(RecurArgs a)
+{
+    __shared__ float tiles[SHARED ? 4 : 1][SEG][WAVE + 1];
+    const Place p = place<1, 4>(a.n);
+    if (p.c0 >= a.n) return;
+    const Shared g(a.gate_span, p), c(a.cut_span, p);
+    const int64_t next = a.reverse ? -a.n : a.n;
+    float2 into = a.dlast ? ((const float2*)a.dlast)[p.c()] : make_float2(0.f, 0.f);
+    for (int64_t i0 = (a.T + SEG - 1) / SEG * SEG - SEG; i0 >= 0; i0 -= SEG) {
+        PairSegment<T, TG, SHARED> s;
+        Two<T> dh[SEG];
+        s.load_gates(a, i0, p, g, c);
+        load_rows(a, (const Two<T>*)a.x, a.n, i0, p.c0, p.l, [&](int k, Two<T> x) { s.v[k] = x; });
+        if (a.dh) load_rows(a, (const Two<T>*)a.dh, a.n, i0, p.c0, p.l, [&](int k, Two<T> x) { dh[k] = x; });
+        const int m = i0 + SEG <= a.T ? SEG : (int)(a.T - i0);
+        float2 before[SEG], h = ((const float2*)a.carry)[i0 / SEG * a.n + p.c()];
+#pragma unroll
+        for (int k = 0; k < SEG; k++) {
+            before[k] = h;
+            if (k >= m) continue;
+            const float2 q = s.at(a, k);
+            h.x = advance(q.x, h.x, (float)s.v[k].a);
+            h.y = advance(q.y, h.y, (float)s.v[k].b);
+        }
+        const int64_t at = step_at(a, i0 + SEG - 1) * a.n + p.c0;
+        Two<T>* row = (Two<T>*)a.dx + at;
+        Two<TG>* gate_row = (Two<TG>*)a.dgate + at;
+        float d[SHARED ? SEG : 1];
+#pragma unroll
+        for (int k = SEG - 1; k >= 0; k--, row -= next, gate_row -= next) {
+            if constexpr (SHARED) d[k] = 0.f;
+            if (k >= m) continue;
+            const float2 q = s.at(a, k);
+            const float gx = into.x + (a.dh ? (float)dh[k].a : 0.f), gy = into.y + (a.dh ? (float)dh[k].b : 0.f);
+            if (p.on) row[p.l] = Two<T>{(T)gx, (T)gy};
+            into.x = advance(q.x, gx, 0.f);
+            into.y = advance(q.y, gy, 0.f);
+            const bool cut = s.cut >> k & 1;
+            const float dx = cut ? 0.f : gx * before[k].x, dy = cut ? 0.f : gy * before[k].y;
+            if constexpr (SHARED) d[k] = dx + dy;
+            else if (a.dgate && p.on) gate_row[p.l] = Two<TG>{(TG)dx, (TG)dy};
+        }
+        if constexpr (SHARED) {
+            if (a.dgate) gate_sums<TG>(a, tiles[threadIdx.x >> 6], i0, p, d);
+        }
+    }
+    if (a.dstate && p.on) ((float2*)a.dstate)[p.c()] = into;
+}
+
 // the waves' parts of every shared gate's sum, in their order
 template <class TG>
 __global__ __launch_bounds__(256) void gate_parts_kernel(RecurArgs a)
@@ -504,6 +615,9 @@ __global__ __launch_bounds__(64 * NW * CW) void advantages_kernel(AdvArgs a, Chu
     if (MAPS && p.w == 0 && p.on) s.maps[blockIdx.y * n + p.c()] = make_float2(whole.a, whole.b);
 }
 
+// parts of a shared gate's sum: the waves that its channels can lie in
+int64_t gate_pieces(int64_t gate_span) { return WAVE % gate_span == 0 ? 1 : (gate_span - 1) / WAVE + 2; }
+
 // How the steps are split.  A wave keeps 2 SEG values a lane in flight; FILL
 // waves keep the memory busy (256 CUs, 16 each), and chunks are made for twice
 // as many: 65537 steps of 96 channels, forward and backward, took 84 us with
@@ -540,9 +654,41 @@ void launch_advantages(const AdvArgs& a, void* workspace, hipStream_t st)
     else hipLaunchKernelGGL((advantages_kernel<TR, TV, 8, 1, false>), grid, dim3(512), 0, st, a, q.s);
 }
 
+bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+// Whether 16-bit channels go in pairs: where channels alone fill the device
+// (20 steps of 1048576 channels bf16, forward and backward: 92 us, 135 us one
+// a lane), pairs share what is shared and nothing lies at odd places.
+template <class T, class TG>
+bool take_pairs(const RecurArgs& a, RecurArgs* b)
+{
+    if (sizeof(T) != 2 || a.n % 2 || split_steps(a.T, a.n, nullptr).nw != 1 || a.n / WAVE / 2 < FILL) return false;
+    const bool shared = !a.gate || a.gate_span > 1;
+    if ((shared && a.gate && a.gate_span % 2) || (a.cut && a.cut_span % 2)) return false;
+    if (!aligned(a.x, 4) || !aligned(a.h, 4) || !aligned(a.dh, 4) || !aligned(a.dx, 4)) return false;
+    if (!shared && (!aligned(a.gate, 2 * sizeof(TG)) || !aligned(a.dgate, 2 * sizeof(TG)))) return false;
+    if (!aligned(a.state, 8) || !aligned(a.last, 8) || !aligned(a.carry, 8) || !aligned(a.dlast, 8) || !aligned(a.dstate, 8))
+        return false;
+    *b = a;
+    b->n = a.n / 2;
+    b->gate_span = shared && a.gate ? a.gate_span / 2 : 1;
+    b->cut_span = a.cut ? a.cut_span / 2 : 1;
+    b->gates = b->n / b->gate_span;
+    b->cuts = b->n / b->cut_span;
+    b->parts = (int32_t)gate_pieces(b->gate_span);
+    return true;
+}
+
 template <class T, class TG>
 void launch_recurrence(const RecurArgs& a, void* workspace, hipStream_t st)
 {
+    RecurArgs b;
+    if constexpr (sizeof(T) == 2) if (take_pairs<T, TG>(a, &b)) {
+        const dim3 blocks((unsigned)((b.n + 4 * WAVE - 1) / (4 * WAVE)));
+        if (!a.gate || a.gate_span > 1) hipLaunchKernelGGL((recur_pair_kernel<T, TG, true>), blocks, dim3(256), 0, st, b);
+        else hipLaunchKernelGGL((recur_pair_kernel<T, TG, false>), blocks, dim3(256), 0, st, b);
+        return;
+    }
     const Split q = split_steps(a.T, a.n, (float2*)workspace);
     const int64_t waves = (a.n + WAVE - 1) / WAVE;
     const dim3 grid((unsigned)waves, q.s.count);
@@ -571,6 +717,15 @@ void launch_backward(const RecurArgs& a, void* workspace, hipStream_t st)
 template <class T, class TG>
 void launch_backward(const RecurArgs& a, void* workspace, hipStream_t st)
 {
+    RecurArgs b;
+    if constexpr (sizeof(T) == 2) if (take_pairs<T, TG>(a, &b)) {
+        const dim3 blocks((unsigned)((b.n + 4 * WAVE - 1) / (4 * WAVE)));
+        if (!a.gate || a.gate_span > 1) hipLaunchKernelGGL((recur_backward_pair_kernel<T, TG, true>), blocks, dim3(256), 0, st, b);
+        else hipLaunchKernelGGL((recur_backward_pair_kernel<T, TG, false>), blocks, dim3(256), 0, st, b);
+        if (b.dgate && a.gate_span > 1 && b.parts > 1)
+            hipLaunchKernelGGL((gate_parts_kernel<TG>), dim3((unsigned)((b.T * b.gates + 255) / 256)), dim3(256), 0, st, b);
+        return;
+    }
     if (a.dgate && a.gate_span > 1) launch_backward<T, TG, true>(a, workspace, st);
     else launch_backward<T, TG, false>(a, workspace, st);
 }
@@ -590,9 +745,6 @@ gw_status check_recurrence(int32_t dtype, int32_t gate_dtype, int64_t T, int64_t
                (long long)n);
     return GW_OK;
 }
-
-// parts of a shared gate's sum: the waves that its channels can lie in
-int64_t gate_pieces(int64_t gate_span) { return WAVE % gate_span == 0 ? 1 : (gate_span - 1) / WAVE + 2; }
 
 int64_t maps_bytes(int64_t T, int64_t n)
 {

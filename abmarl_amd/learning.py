@@ -169,6 +169,13 @@ def _call(fn, device, *args):
         _native.check_learn(st, fn.__name__)
 
 
+def _once():
+    # (autograd runs a backward pass with gradients off unless it is to be
+    # differentiated itself)
+    if torch.is_grad_enabled():
+        raise RuntimeError("the policy operators' gradients cannot be differentiated again (create_graph)")
+
+
 # ------------------------------------------------------------------ sampling
 def sample_actions(logits, heads, noise=None, choice_mask=None, out=None):
     """Draws an action row for each row of logits [..., n_choices] (float32,
@@ -267,8 +274,8 @@ class _PolicyLoss(torch.autograd.Function):
         return out.select(0, 0).detach(), out, logp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_loss, _out, _logp):
+        _once()
         logits, actions, advantage, old_logp, ref, valid, mask, at, out = ctx.saved_tensors
         heads, args, kl_coef, entropy_coef = ctx.rest
         if d_loss is None:
@@ -370,8 +377,8 @@ class _Recurrence(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dlast):
+        _once()
         gate, x, cut, carry = ctx.saved_tensors
         value, gate_span, cut_span, reverse, has_state = ctx.rest
         if dh is None and dlast is None:

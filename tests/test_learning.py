@@ -539,6 +539,34 @@ def test_recurrence_backward(shape, dtype):
 
 
 @gpu
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('shape,gk,ck,reverse', [
+    ((18, 2048, 258), 'full', 'envs', False), ((18, 2048, 258), 'shared', 'envs', True),
+    ((16, 4096, 130), 'f32', 'none', True), ((3, 4096, 130), 'steps', 'none', False),
+    ((5, 4096, 129), 'shared', 'envs', False), ((1, 524288, 1), 'full', 'none', False),
+    ((2, 262144, 2), 'shared', 'full', False)])
+def test_recurrence_many_channels(shape, gk, ck, reverse, dtype):
+    """So many channels that they alone fill the device: pairs of 16-bit
+    channels, and what cannot be paired (odd spans, a cut for each channel)."""
+    gate, x, state, cut, g = recurrence_inputs(shape, dtype, gk, ck, 20)
+    dh, dlast = torch.randn(shape, generator=g).to(dtype), torch.randn(shape[1:], generator=g)
+    want, last = ref.recurrence(gate, x, state, cut, reverse)
+    e, e_last = ref.recurrence_error(gate, x, state, cut, reverse)
+    (wg, wx, ws), e_gate, e_x, e_s = _gradients(gate, x, state, cut, reverse, dh, dlast)
+    leaves = [t.cuda().requires_grad_() for t in (gate, x, state)]
+    h, l = learning.linear_recurrence(*leaves, cut=None if cut is None else cut.cuda(), reverse=reverse)
+    dg, dx, ds = torch.autograd.grad((h, l), leaves, (dh.cuda(), dlast.cuda()))
+    assert ref.near(h, want.detach(), e, dtype) <= 1 and ref.near(l, last.detach(), e_last) <= 1
+    assert ref.near(dx, wx, e_x, dtype) <= 1 and ref.near(ds, ws, e_s) <= 1
+    assert ref.near(dg, wg, e_gate, gate.dtype) <= 1
+    if gk == 'full':                                             # a gate of one number, no state
+        want, last = ref.recurrence(0.9, x, None, cut, reverse)
+        e, _ = ref.recurrence_error(0.9, x, None, cut, reverse)
+        h, _ = learning.linear_recurrence(0.9, x.cuda(), cut=None if cut is None else cut.cuda(), reverse=reverse)
+        assert ref.near(h, want, e, dtype) <= 1
+
+
+@gpu
 def test_recurrence_partial_gradients():
     """Only h or only last has a gradient; leaves that need none; an expanded
     gradient (of a sum)."""
