@@ -138,7 +138,7 @@ LEARN_SIGNATURES = {
     'gw_policy_sample': (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     'gw_policy_loss_workspace': (_i64, [_i64]),
     'gw_policy_loss': (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64,
-                              _f32, _f32, _f32, _f32, _f32, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+                              _f32, _f32, _f32, _f32, _f32, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     'gw_recurrence_workspace': (_i64, [_i64, _i64]),
     'gw_recurrence': (_i32, [_i32, _i32, _i64, _i64, _vp, _vp, _i64, _f32, _vp, _i64, _vp, _i32,
                              _vp, _vp, _vp, _vp, _i64, _vp]),

@@ -41,7 +41,7 @@ struct LossArgs {
     float lo, hi, kl, entropy;                  // 1 - clip_low, 1 + clip_high, coefficients
     float denominator; const float* denominator_at;
     float scale; const float* upstream;
-    float* out; float* logp; void* grad;
+    float* out; float* stats; float* logp; void* grad;      // out: the loss
     const int32_t* counts; int32_t n_counts;    // valid rows per block of count_kernel
     double* partial;                            // [blocks][N_SUMS]
 };
@@ -233,18 +233,18 @@ __device__ __forceinline__ float inverse_rows(const LossArgs& a)
     return m > 0.f ? 1.f / m : 0.f;
 }
 
-// the blocks' sums to the six numbers of gw_policy_loss's out
+// the blocks' sums to gw_policy_loss's loss and stats
 __device__ __forceinline__ void write_out(const LossArgs& a, const double* s)
 {
     const float given = a.denominator > 0.f ? a.denominator : a.denominator_at ? *a.denominator_at : -1.f;
     const double m = given >= 0.f ? (double)given : s[S_COUNT];
     const double inv = m > 0. ? 1. / m : 0.;
     a.out[0] = (float)((s[S_PG] + (double)a.kl * s[S_KL] - (double)a.entropy * s[S_H]) * inv);
-    a.out[1] = (float)(s[S_PG] * inv);
-    a.out[2] = (float)(s[S_KL] * inv);
-    a.out[3] = (float)(s[S_H] * inv);
-    a.out[4] = (float)(s[S_CLIP] * inv);
-    a.out[5] = (float)m;
+    a.stats[0] = (float)(s[S_PG] * inv);
+    a.stats[1] = (float)(s[S_KL] * inv);
+    a.stats[2] = (float)(s[S_H] * inv);
+    a.stats[3] = (float)(s[S_CLIP] * inv);
+    a.stats[4] = (float)m;
 }
 
 // ------------------------------------------------------------ rows out of registers
@@ -946,7 +946,7 @@ struct Rows {
 };
 
 template <class T, int V, int L>
-__global__ __launch_bounds__(L ? 256 : 1024) void sample_wide_kernel(SampleArgs a, OneHead h)
+__global__ __launch_bounds__(L ? 256 : V == 8 ? 512 : 1024) void sample_wide_kernel(SampleArgs a, OneHead h)
 {
     __shared__ float box[2][16];
     __shared__ float best_s[16];
@@ -1034,7 +1034,7 @@ __global__ __launch_bounds__(L ? 256 : 1024) void sample_wide_kernel(SampleArgs 
 }
 
 template <class T, int V, int L, bool REF, bool GRAD>
-__global__ __launch_bounds__(L ? 256 : 1024) void loss_wide_kernel(LossArgs a, OneHead h)
+__global__ __launch_bounds__(L ? 256 : V == 8 ? 512 : 1024) void loss_wide_kernel(LossArgs a, OneHead h)
 {
     __shared__ float box[4][16];
     typedef WideRow<T, V, L> Row;
@@ -1429,17 +1429,20 @@ void launch_sample_narrow(const SampleArgs& a, const Small& s, hipStream_t st)
 }
 
 // How a wide head's rows are shared out, or false where registers do not hold
-// them: pieces of 16 bytes, one or (from 256 on) four a lane; fewer than a
-// wave's lanes a row where the row has fewer pieces.
+// them: pieces of 16 bytes, one or (from 65 pieces on) four a lane; fewer than a
+// wave's lanes a row where the row has fewer pieces.  Above 1024 pieces the loss
+// takes eight a lane: fewer waves a row hold fewer copies of what is not the
+// row, so three rows fit a CU in place of two (4099 x 12800 bf16: 119 us, 130 us
+// with four; drawing, which holds one row and its noise, 27 us against 24).
 struct WideSplit { int v, lanes, threads; };
 
-bool take_wide(const Heads& h, int size, WideSplit* w)
+bool take_wide(const Heads& h, int size, bool loss, WideSplit* w)
 {
     if (h.n != 1 || h.width <= NARROW) return false;
     const int pieces = (h.width * size + 15) / 16;
-    w->v = pieces > 64 ? 4 : 1;
+    w->v = pieces > (loss ? 1024 : 4096) ? 8 : pieces > 64 ? 4 : 1;
     const int lanes = (pieces + w->v - 1) / w->v;
-    if (lanes > 1024) return false;
+    if (lanes > (w->v == 8 ? 512 : 1024)) return false;
     w->lanes = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : lanes <= 64 ? 64 : 0;
     w->threads = w->lanes ? 256 : (lanes + 63) / 64 * 64;
     return true;
@@ -1471,10 +1474,11 @@ template <class T>
 void launch_sample(const SampleArgs& a, const Heads& h, hipStream_t st)
 {
     WideSplit w;
-    if (take_wide(h, sizeof(T), &w)) {
+    if (take_wide(h, sizeof(T), false, &w)) {
         const OneHead o{h.width, h.low[0], h.slot[0], h.act_dim};
         if (w.v == 1) launch_sample_wide<T, 1>(a, o, w, st);
-        else launch_sample_wide<T, 4>(a, o, w, st);
+        else if (w.v == 4) launch_sample_wide<T, 4>(a, o, w, st);
+        else hipLaunchKernelGGL((sample_wide_kernel<T, 8, 0>), dim3(wide_blocks(w, a.rows)), dim3(w.threads), 0, st, a, o);
         return;
     }
     Small s;
@@ -1531,7 +1535,7 @@ template <class T>
 unsigned launch_loss(const LossArgs& a, const Heads& h, hipStream_t st)
 {
     WideSplit w;
-    if (take_wide(h, sizeof(T), &w)) {
+    if (take_wide(h, sizeof(T), true, &w)) {
         const OneHead o{h.width, h.low[0], h.slot[0], h.act_dim};
         const unsigned blocks = wide_blocks(w, a.rows);
         if (w.v == 1) {
@@ -1539,7 +1543,8 @@ unsigned launch_loss(const LossArgs& a, const Heads& h, hipStream_t st)
             else if (w.lanes == 16) launch_loss_wide<T, 1, 16>(a, o, blocks, w.threads, st);
             else if (w.lanes == 32) launch_loss_wide<T, 1, 32>(a, o, blocks, w.threads, st);
             else launch_loss_wide<T, 1, 64>(a, o, blocks, w.threads, st);
-        } else if (w.lanes == 32) launch_loss_wide<T, 4, 32>(a, o, blocks, w.threads, st);
+        } else if (w.v == 8) launch_loss_wide<T, 8, 0>(a, o, blocks, w.threads, st);
+        else if (w.lanes == 32) launch_loss_wide<T, 4, 32>(a, o, blocks, w.threads, st);
         else if (w.lanes == 64) launch_loss_wide<T, 4, 64>(a, o, blocks, w.threads, st);
         else launch_loss_wide<T, 4, 0>(a, o, blocks, w.threads, st);
         return blocks;
@@ -1620,7 +1625,7 @@ gw_status gw_policy_loss(const gw_policy_heads* heads, int32_t dtype, int64_t n_
                          float clip_low, float clip_high, float kl_coef, float entropy_coef,
                          float denominator, const float* denominator_at,
                          float grad_scale, const float* upstream,
-                         float* out, float* logp, void* grad,
+                         float* loss, float* stats, float* logp, void* grad,
                          void* workspace, int64_t workspace_bytes, void* stream)
 {
     Heads h;
@@ -1633,21 +1638,22 @@ gw_status gw_policy_loss(const gw_policy_heads* heads, int32_t dtype, int64_t n_
                "clip %g, %g: finite and not negative", clip_low, clip_high);
     LEARN_NEED(isfinite(kl_coef) && isfinite(entropy_coef) && isfinite(grad_scale) && isfinite(denominator),
                "a coefficient is not finite");
-    LEARN_NEED(out || logp || grad || n_rows == 0, "nothing to compute: out, logp and grad are null");
+    LEARN_NEED(!loss == !stats, "loss and stats: both or neither");
+    LEARN_NEED(loss || logp || grad || n_rows == 0, "nothing to compute: loss, logp and grad are null");
     LEARN_NEED(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= gw_policy_loss_workspace(n_rows),
                "workspace: %lld bytes, 8-byte aligned, are needed", (long long)gw_policy_loss_workspace(n_rows));
     const hipStream_t st = (hipStream_t)stream;
     LossArgs a{};
-    a.logits = logits; a.ref = kl_coef == 0.f && !out ? nullptr : ref; a.ld = ld; a.ld_ref = ld_ref; a.rows = n_rows;
+    a.logits = logits; a.ref = kl_coef == 0.f && !loss ? nullptr : ref; a.ld = ld; a.ld_ref = ld_ref; a.rows = n_rows;
     a.actions = actions; a.advantage = advantage; a.old_logp = old_logp;
     a.valid = valid; a.mask = choice_mask; a.mask_rows = mask_rows;
     a.lo = 1.f - clip_low; a.hi = 1.f + clip_high; a.kl = kl_coef; a.entropy = entropy_coef;
     a.denominator = denominator; a.denominator_at = denominator_at;
     a.scale = grad_scale; a.upstream = upstream;
-    a.out = out; a.logp = logp; a.grad = grad;
+    a.out = loss; a.stats = stats; a.logp = logp; a.grad = grad;
     a.partial = (double*)workspace;
     if (n_rows == 0) {
-        if (out) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(2 * N_SUMS * WAVE), 0, st, a, 0);
+        if (loss) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(2 * N_SUMS * WAVE), 0, st, a, 0);
         LEARN_LAUNCHED();
         return GW_OK;
     }
@@ -1661,7 +1667,7 @@ gw_status gw_policy_loss(const gw_policy_heads* heads, int32_t dtype, int64_t n_
     }
     const unsigned blocks = dtype == GW_T_F32 ? launch_loss<float>(a, h, st)
                           : dtype == GW_T_F16 ? launch_loss<f16>(a, h, st) : launch_loss<bf16>(a, h, st);
-    if (out && blocks > 1) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(2 * N_SUMS * WAVE), 0, st, a, (int)blocks);
+    if (loss && blocks > 1) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(2 * N_SUMS * WAVE), 0, st, a, (int)blocks);
     LEARN_LAUNCHED();
     return GW_OK;
 }

@@ -249,7 +249,7 @@ def _finite(name, v):
 
 
 def _launch_loss(logits, actions, advantage, old_logp, ref, valid, heads, args, kl_coef, entropy_coef,
-                 grad_scale=1.0, upstream=None, out=None, logp=None, grad=None, denominator_at=None):
+                 grad_scale=1.0, upstream=None, loss=None, stats=None, logp=None, grad=None, denominator_at=None):
     n, ld, ld_ref, mask, mask_rows, low, high, value, at = args
     L, device = _lib(), logits.device
     size = L.gw_policy_loss_workspace(n)
@@ -257,32 +257,37 @@ def _launch_loss(logits, actions, advantage, old_logp, ref, valid, heads, args, 
     _call(L.gw_policy_loss, device, heads._p, _DTYPES[logits.dtype], n, logits.data_ptr(), ld, _at(ref), ld_ref,
           actions.data_ptr(), advantage.data_ptr(), old_logp.data_ptr(), _at(valid), _at(mask), mask_rows, low, high,
           kl_coef, entropy_coef, value, _at(at if denominator_at is None else denominator_at), grad_scale,
-          _at(upstream), _at(out), _at(logp), _at(grad), work.data_ptr(), size)
+          _at(upstream), _at(loss), _at(stats), _at(logp), _at(grad), work.data_ptr(), size)
+
+
+def _loss_outputs(logits):
+    device = logits.device
+    return (torch.empty((), dtype=torch.float32, device=device), torch.empty(5, dtype=torch.float32, device=device),
+            torch.empty(logits.shape[:-1], dtype=torch.float32, device=device))
 
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, advantage, old_logp, ref, valid, mask, at, heads, args, kl_coef, entropy_coef):
-        out = torch.empty(6, dtype=torch.float32, device=logits.device)
-        logp = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+        loss, stats, logp = _loss_outputs(logits)
         _launch_loss(logits, actions, advantage, old_logp, ref, valid, heads, args, kl_coef, entropy_coef,
-                     out=out, logp=logp)
-        ctx.save_for_backward(logits, actions, advantage, old_logp, ref, valid, mask, at, out)
+                     loss=loss, stats=stats, logp=logp)
+        ctx.save_for_backward(logits, actions, advantage, old_logp, ref, valid, mask, at, stats)
         ctx.rest = heads, args, kl_coef, entropy_coef
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(out, logp)
-        return out.select(0, 0).detach(), out, logp
+        ctx.mark_non_differentiable(stats, logp)
+        return loss, stats, logp
 
     @staticmethod
-    def backward(ctx, d_loss, _out, _logp):
+    def backward(ctx, d_loss, _stats, _logp):
         _once()
-        logits, actions, advantage, old_logp, ref, valid, mask, at, out = ctx.saved_tensors
+        logits, actions, advantage, old_logp, ref, valid, mask, at, stats = ctx.saved_tensors
         heads, args, kl_coef, entropy_coef = ctx.rest
         if d_loss is None:
             return (None,) * 12
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         _launch_loss(logits, actions, advantage, old_logp, ref, valid, heads, args, kl_coef, entropy_coef,
-                     upstream=d_loss.contiguous(), grad=grad, denominator_at=out[5])
+                     upstream=d_loss.contiguous(), grad=grad, denominator_at=stats[4])
         return (grad,) + (None,) * 11
 
 
@@ -313,9 +318,9 @@ def policy_loss(logits, actions, advantage, old_logp, heads, *, ref_logits=None,
     args = _loss_args(logits, actions, advantage, old_logp, heads, ref_logits, valid, choice_mask, clip, denominator)
     kl_coef, entropy_coef = _finite('kl_coef', kl_coef), _finite('entropy_coef', entropy_coef)
     _gpu(logits.device)
-    loss, out, logp = _PolicyLoss.apply(logits, actions, advantage, old_logp, ref_logits, valid, args[3], args[8],
-                                        heads, args, kl_coef, entropy_coef)
-    return PolicyLoss(loss, out[1:5], out[5], logp)
+    loss, stats, logp = _PolicyLoss.apply(logits, actions, advantage, old_logp, ref_logits, valid, args[3], args[8],
+                                          heads, args, kl_coef, entropy_coef)
+    return PolicyLoss(loss, stats[:4], stats[4], logp)
 
 
 def policy_loss_grad(logits, actions, advantage, old_logp, heads, *, ref_logits=None, valid=None, choice_mask=None,
@@ -329,12 +334,11 @@ def policy_loss_grad(logits, actions, advantage, old_logp, heads, *, ref_logits=
     grad_scale = _finite('grad_scale', grad_scale)
     device = logits.device
     _gpu(device)
-    out = torch.empty(6, dtype=torch.float32, device=device)
-    logp = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
+    loss, stats, logp = _loss_outputs(logits)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
     _launch_loss(logits, actions, advantage, old_logp, ref_logits, valid, heads, args, kl_coef, entropy_coef,
-                 grad_scale=grad_scale, out=out, logp=logp, grad=grad)
-    return PolicyGradient(out[0], out[1:5], out[5], logp, grad)
+                 grad_scale=grad_scale, loss=loss, stats=stats, logp=logp, grad=grad)
+    return PolicyGradient(loss, stats[:4], stats[4], logp, grad)
 
 
 # ---------------------------------------------------------------- recurrence

@@ -78,8 +78,9 @@ gw_status gw_policy_sample(const gw_policy_heads* heads, int32_t dtype, int64_t 
      loss = 1/M sum over valid rows of
             - min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A)
             + kl_coef KL(q || p) - entropy_coef H(p)
-     out      float [6]: loss, and the means over valid rows of the policy
-              term, KL, entropy and the share of clipped rows; M.  NULL: none
+     loss     float [1];  stats  float [5]: the means over valid rows of the
+              policy term, KL, entropy and clipped rows, and M.  Both or
+              neither NULL
      logp     float [n_rows]: L (0 for rows not valid); NULL: not wanted
      grad     [n_rows][n_choices] of dtype, rows side by side: dloss/dlogits
               times grad_scale (and times *upstream); 0 for rows not valid
@@ -101,7 +102,7 @@ gw_status gw_policy_loss(const gw_policy_heads* heads, int32_t dtype, int64_t n_
                          float clip_low, float clip_high, float kl_coef, float entropy_coef,
                          float denominator, const float* denominator_at,
                          float grad_scale, const float* upstream,
-                         float* out, float* logp, void* grad,
+                         float* loss, float* stats, float* logp, void* grad,
                          void* workspace, int64_t workspace_bytes, void* stream);
 
 /* h[t] = (cut[t] ? 0 : gate[t] h[t-1]) + x[t] for t = 0..n_steps-1, h[-1] =

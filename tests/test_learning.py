@@ -161,11 +161,11 @@ def test_c_entries_refuse_without_a_gpu():
         (L.gw_policy_sample, (heads, 0, 4, one, 8, None, one, 3, one, None, None, None), 'mask'),
         (L.gw_policy_sample, (heads, 0, 4, one, 8, None, None, 0, None, None, None, None), 'actions')]
     loss = [heads, 0, 4, one, 8, None, 0, one, one, one, None, None, 0, 0.2, 0.2, 0.0, 0.0, 0.0, None, 1.0, None,
-            one, one, one, one, 1 << 20, None]
-    for i, v, word in [(7, None, 'actions'), (13, -1.0, 'clip'), (15, math.nan, 'coefficient'), (24, None, 'workspace'),
-                       (25, 8, 'workspace'), (24, C.c_void_p(12), 'workspace')]:
+            one, one, one, one, one, 1 << 20, None]
+    for i, v, word in [(7, None, 'actions'), (13, -1.0, 'clip'), (15, math.nan, 'coefficient'), (25, None, 'workspace'),
+                       (26, 8, 'workspace'), (25, C.c_void_p(12), 'workspace'), (22, None, 'both')]:
         bad.append((L.gw_policy_loss, loss[:i] + [v] + loss[i + 1:], word))
-    bad.append((L.gw_policy_loss, loss[:21] + [None, None, None] + loss[24:], 'nothing'))
+    bad.append((L.gw_policy_loss, loss[:21] + [None, None, None, None] + loss[25:], 'nothing'))
     rec = [0, 0, 3, 4, one, one, 1, 0.0, None, 1, None, 0, one, one, None, one, 1 << 30, None]
     for i, v, word in [(0, 5, 'dtype'), (1, 2, 'gate_dtype'), (2, -1, 'steps'), (4, None, 'x'), (6, 3, 'gate_span'),
                        (12, None, 'h')]:
