@@ -77,6 +77,10 @@ SIGNATURES = {
 }
 
 
+# no packed-fp32 instructions: some of their forms have given wrong results
+NO_PACKED = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+
+
 PART_SIDES = (1, 3, 5, 7, 9, 11, 13, 15, 0)   # observation window sides S = 2*range+1; 0: any S > 15
 
 
@@ -97,7 +101,7 @@ def build(force=False, verbose=False, stamps=False, checks=False, out=None, extr
     if extra_flags:   # tools' A/B builds (tools/ab_lib.py)
         tag = os.path.splitext(os.path.basename(out))[0]
     flags = [f'--offload-arch={ARCH}', '-O3', '-std=c++17', '-ffp-contract=off', '-fPIC',
-             '-Wno-unused-result'] + (['-DGW_STAMPS'] if stamps else []) + \
+             '-Wno-unused-result'] + NO_PACKED + (['-DGW_STAMPS'] if stamps else []) + \
         (['-DGW_CHECKS'] if checks else []) + list(extra_flags)
     objdir = os.path.join(os.path.dirname(out), f'obj_{tag}')
     os.makedirs(objdir, exist_ok=True)
@@ -165,8 +169,8 @@ def build_learn(force=False, verbose=False, out=None, extra_flags=()):
     objdir = os.path.join(os.path.dirname(out), 'obj_' + os.path.splitext(os.path.basename(out))[0])
     os.makedirs(objdir, exist_ok=True)
     objs = [os.path.join(objdir, os.path.basename(s)[:-4] + '.o') for s in LEARN_SRCS]
-    cmds = [[HIPCC, f'--offload-arch={ARCH}', '-O3', '-std=c++17', '-fPIC', '-Wno-unused-result',
-             '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops'] + list(extra_flags) +
+    cmds = [[HIPCC, f'--offload-arch={ARCH}', '-O3', '-std=c++17', '-fPIC', '-Wno-unused-result'] +
+            NO_PACKED + list(extra_flags) +
             ['-c', '-o', o, s] for s, o in zip(LEARN_SRCS, objs)]
     link = [HIPCC, f'--offload-arch={ARCH}', '-shared', '-fPIC', '-o', out + '.tmp'] + objs
     if verbose:

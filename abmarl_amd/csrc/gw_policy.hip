@@ -606,6 +606,8 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
 {
     extern __shared__ float4 lds[];
     constexpr int PLANES = REF ? 5 : 3;
+    // wide rows' exponentials are made again for the gradient: kept, they cost a third of the waves
+    constexpr bool KEEP = GRAD && CM < 32;
     typedef typename std::conditional<(CM > 32), uint64_t, uint32_t>::type Picks;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     // per wave: [heads][PLANES][64] sums, then the tile of gradients
@@ -648,7 +650,7 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
         const int64_t base = at_row.base;
         const uint32_t l = at_row.l;
         const Bounds heads(h);
-        float x[CM], y[REF ? CM : 1], e[CM];
+        float x[CM], y[REF ? CM : 1], e[KEEP ? CM : 1];
         next.z.get(heads.width, x);
         if constexpr (REF) next.r.get(heads.width, y);
         const bool there = at_row.there, valid = there && next.valid;
@@ -696,16 +698,17 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
 #pragma unroll
         for (int j = 0; j < CM; j++) {
             const float on = __uint_as_float(0x3f800000u * (1u - (uint32_t)(heads.starts >> j & 1)));
-            e[j] = exp2_of(x[j]);
-            s = fmaf(on, s, e[j]);
-            t = fmaf(on, t, e[j] * x[j]);
+            const float ej = exp2_of(x[j]);
+            if constexpr (KEEP) e[j] = ej;
+            s = fmaf(on, s, ej);
+            t = fmaf(on, t, ej * x[j]);
             const uint32_t pick = 0u - (uint32_t)(picks >> j & 1);
             at = fmaf(on, at, __uint_as_float(pick & __float_as_uint(x[j])));
             if constexpr (REF) {
                 const float er = exp2_of(y[j]);
                 sr = fmaf(on, sr, er);
                 u = fmaf(on, u, er * (y[j] - x[j]));
-                y[j] = er;
+                if constexpr (KEEP) y[j] = er;
             }
             if (bit(heads.ends, j)) {
                 plane[P_S * WAVE] = s;
@@ -762,6 +765,9 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
             asm volatile("" : "+v"(picks));
 #pragma unroll
             for (int j = 0; j < CM; j++) asm volatile("" : "+v"(x[j]));
+            if constexpr (REF && !KEEP)
+#pragma unroll
+                for (int j = 0; j < CM; j++) asm volatile("" : "+v"(y[j]));
             plane = planes;
 #pragma unroll
             for (int j = 0; j < CM; j++) {
@@ -773,8 +779,9 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
                     plane += PLANES * WAVE;
                 }
                 // (e x is 0 for choices far below, where a1 x may overflow)
-                float g = fmaf(a1, e[j] * x[j], e[j] * a0);
-                if constexpr (REF) g = fmaf(b, y[j], g);
+                const float ej = KEEP ? e[KEEP ? j : 0] : exp2_of(x[j]);
+                float g = fmaf(a1, ej * x[j], ej * a0);
+                if constexpr (REF) g = fmaf(b, KEEP ? y[j] : exp2_of(y[j]), g);
                 const uint32_t pick = 0u - (uint32_t)(picks >> j & 1);
                 g += __uint_as_float(pick & __float_as_uint(pull));
                 x[j] = valid && x[j] != NO_CHOICE ? g : 0.f;

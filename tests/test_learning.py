@@ -442,6 +442,111 @@ def test_policy_loss_gradient_against_differences():
     assert abs((up64['loss'] - dn64['loss']) / (2 * h) - slope) < 1e-3 * float(v.norm())
 
 
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('name,N,lanes', [('team', 700, 7), ('team', 1000, 100), ('rtt', 640, 64), ('odd', 130, 130),
+                                          ('w65', 90, 30), ('w513', 12, 4), ('cells', 12, 3)])
+def test_lane_masks_wrap(name, N, lanes, dtype):
+    """Mask rows that repeat inside and across tiles of rows."""
+    heads = LAYOUTS[name]
+    g = gen(N + lanes)
+    z = torch.randn(N, heads.n_choices, generator=g).to(dtype)
+    mask = (torch.rand(lanes, heads.n_choices, generator=g) < 0.6).to(torch.uint8)
+    noise = gumbel(z.shape, g)
+    act, logp, _, e, _ = ref.sample(z, heads, noise, mask.repeat(N // lanes, 1))
+    got = learning.sample_actions(z.cuda(), heads, noise.cuda(), mask.cuda())
+    assert got.actions.cpu().equal(act) and ref.near(got.logp, logp, e) <= 1
+    old = (logp + 0.1).float()
+    adv = torch.randn(N, generator=g)
+    want = ref.policy_loss(z, act, adv, old, heads, z, None, mask, kl_coef=0.1, entropy_coef=0.01)
+    zc, actc, advc, oldc, mc = cuda(z, act, adv, old, mask)
+    got = learning.policy_loss_grad(zc, actc, advc, oldc, heads, ref_logits=zc, choice_mask=mc, kl_coef=0.1,
+                                    entropy_coef=0.01)
+    check_loss(got, want, dtype)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('name', ['team', 'rtt', 'odd', 'w65', 'w513', 'w4100', 'mixed'])
+def test_odd_addresses_and_strides(name, dtype):
+    """Rows that begin at any element and lie any stride apart; a gradient is
+    still side by side."""
+    heads = LAYOUTS[name]
+    g = gen(7)
+    N, Cn = 5, heads.n_choices
+    for shift, pad in ((1, 0), (3, 1), (0, 7)):
+        flat = torch.full((shift + N * (Cn + pad),), math.nan, dtype=dtype)
+        z = torch.randn(N, Cn, generator=g).to(dtype)
+        view = flat[shift:].view(N, Cn + pad)[:, :Cn]
+        view.copy_(z)
+        zc = flat.cuda()[shift:].view(N, Cn + pad)[:, :Cn]
+        noise = gumbel(z.shape, g)
+        act, logp, _, e, _ = ref.sample(z, heads, noise)
+        got = learning.sample_actions(zc, heads, noise.cuda())
+        assert got.actions.cpu().equal(act) and ref.near(got.logp, logp, e) <= 1
+        adv, old = torch.randn(N, generator=g), (logp - 0.05).float()
+        want = ref.policy_loss(z, act, adv, old, heads, z, None, None, kl_coef=0.1, entropy_coef=0.01)
+        got = learning.policy_loss_grad(zc, *cuda(act, adv, old), heads, ref_logits=zc, kl_coef=0.1, entropy_coef=0.01)
+        check_loss(got, want, dtype)
+
+
+@gpu
+def test_masked_by_the_lowest_value():
+    """Choices masked by their type's lowest number, as some policies do, with
+    a large loss scale: probability 0, gradient 0, nothing infinite."""
+    for name in ('team', 'rtt', 'w65', 'w4100', 'cells'):
+        heads = LAYOUTS[name]
+        for dtype in DTYPES:
+            g = gen(5)
+            z = torch.randn(6, heads.n_choices, generator=g)
+            hide = torch.rand(z.shape, generator=g) < 0.4
+            for s in ref.head_slices(heads):
+                hide[:, s.start] = False
+            low = torch.finfo(dtype).min
+            zl = torch.where(hide, low, z.to(dtype).float()).to(dtype)
+            mask = (~hide).to(torch.uint8)
+            act, logp, _, _, _ = ref.sample(z.to(dtype), heads, None, mask)
+            args = cuda(act, torch.randn(6, generator=g), logp.float())
+            kw = dict(entropy_coef=0.1, grad_scale=2.0 ** 14, denominator=1.0)
+            a = learning.policy_loss_grad(zl.cuda(), *args, heads, **kw)
+            b = learning.policy_loss_grad(z.to(dtype).cuda(), *args, heads, choice_mask=mask.cuda(), **kw)
+            assert torch.isfinite(a.grad.float()).all().item() and torch.isfinite(a.loss).item()
+            assert not a.grad.cpu()[hide].any().item()
+            size = float(b.grad.float().abs().max())
+            assert (a.grad.float() - b.grad.float()).abs().max().item() <= size * (2.0 ** -18 + torch.finfo(dtype).eps)
+
+
+@gpu
+def test_more_than_two_to_the_31_elements():
+    """Offsets past 32 bits: the last rows and channels as on their own."""
+    N = (1 << 28) + 130
+    z = torch.zeros(N, 8, dtype=torch.bfloat16, device='cuda')
+    tail = torch.randn(130, 8, generator=gen(1)).bfloat16().cuda()
+    z[-130:] = tail
+    act = torch.zeros(N, 3, dtype=torch.int32, device='cuda')
+    adv = torch.ones(N, device='cuda')
+    old = torch.zeros(N, device='cuda')
+    got = learning.policy_loss_grad(z, act, adv, old, TEAM, entropy_coef=0.1, denominator=1.0)
+    own = learning.policy_loss_grad(tail, act[-130:], adv[-130:], old[-130:], TEAM, entropy_coef=0.1, denominator=1.0)
+    assert got.grad[-130:].equal(own.grad) and got.logp[-130:].equal(own.logp) and got.count.item() == 1.0
+    del got
+    r = learning.sample_actions(z, TEAM, out=act)
+    assert r.actions[-130:].equal(learning.sample_actions(tail, TEAM).actions)
+    del z, r, act, adv, old
+    wide = torch.zeros(170000, 12801, dtype=torch.bfloat16, device='cuda')
+    heads = PolicyHeads([12801])
+    wide[-3:] = torch.randn(3, 12801, generator=gen(2)).bfloat16().cuda()
+    assert learning.sample_actions(wide, heads).actions[-3:].equal(learning.sample_actions(wide[-3:].clone(), heads).actions)
+    del wide
+    n = 1 << 29
+    x = torch.zeros(5, n, dtype=torch.bfloat16, device='cuda')
+    part = torch.randn(5, 200, generator=gen(3)).bfloat16().cuda()
+    x[:, -200:] = part
+    h, last = learning.linear_recurrence(0.5, x)
+    own, own_last = learning.linear_recurrence(0.5, part)
+    assert h[:, -200:].equal(own) and last[-200:].equal(own_last)
+
+
 # ----------------------------------------------------------- GPU: recurrence
 SHAPES = [(1, 1), (1, 7), (2, 64), (15, 3), (16, 65), (17, 130), (33, 2, 5), (100, 4, 3, 2), (257, 96), (1000, 2),
           (4099, 5), (40, 300, 17)]
