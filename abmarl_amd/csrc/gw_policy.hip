@@ -218,25 +218,32 @@ __device__ __forceinline__ RowLoss row_loss(const LossArgs& a, float adv, float 
     return r;
 }
 
+// M as it is given, or -1: the valid rows are to be counted
+__device__ __forceinline__ float given_rows(const LossArgs& a)
+{
+    return a.denominator > 0.f ? a.denominator : a.denominator_at ? fmaxf(*a.denominator_at, 0.f) : -1.f;
+}
+
 // 1/M, or 0 where there is nothing to take a mean of
 __device__ __forceinline__ float inverse_rows(const LossArgs& a)
 {
-    if (a.denominator > 0.f) return 1.f / a.denominator;
-    float m;
-    if (a.denominator_at) m = *a.denominator_at;
-    else if (a.counts) {
-        // (every wave adds the blocks' counts: fewer than 2^31 rows a block)
-        int64_t n = 0;
-        for (int i = threadIdx.x & 63; i < a.n_counts; i += WAVE) n += a.counts[i];
-        m = (float)wave_sum(n);
-    } else m = (float)a.rows;
+    float m = given_rows(a);
+    if (m < 0.f) {
+        m = (float)a.rows;
+        if (a.counts) {
+            // (every wave adds the blocks' counts)
+            int64_t n = 0;
+            for (int i = threadIdx.x & 63; i < a.n_counts; i += WAVE) n += a.counts[i];
+            m = (float)wave_sum(n);
+        }
+    }
     return m > 0.f ? 1.f / m : 0.f;
 }
 
 // the blocks' sums to gw_policy_loss's loss and stats
 __device__ __forceinline__ void write_out(const LossArgs& a, const double* s)
 {
-    const float given = a.denominator > 0.f ? a.denominator : a.denominator_at ? *a.denominator_at : -1.f;
+    const float given = given_rows(a);
     const double m = given >= 0.f ? (double)given : s[S_COUNT];
     const double inv = m > 0. ? 1. / m : 0.;
     a.out[0] = (float)((s[S_PG] + (double)a.kl * s[S_KL] - (double)a.entropy * s[S_H]) * inv);
@@ -953,7 +960,7 @@ struct Rows {
 };
 
 template <class T, int V, int L>
-__global__ __launch_bounds__(L ? 256 : V == 8 ? 512 : 1024) void sample_wide_kernel(SampleArgs a, OneHead h)
+__global__ __launch_bounds__(L ? 256 : 1024) void sample_wide_kernel(SampleArgs a, OneHead h)
 {
     __shared__ float box[2][16];
     __shared__ float best_s[16];
@@ -1060,7 +1067,7 @@ __global__ __launch_bounds__(L ? 256 : V == 8 ? 512 : 1024) void loss_wide_kerne
         const int pieces = Row::pieces(h.width);
         z.load(zrow, h.width, pieces);
         if constexpr (REF) r.load((const T*)a.ref + row * a.ld_ref, h.width, pieces);
-        const int c = a.actions[row * h.act_dim + h.slot] - h.low;
+        const int c = (int)((uint32_t)a.actions[row * h.act_dim + h.slot] - (uint32_t)h.low);
         const bool inside = (uint32_t)c < (uint32_t)h.width;
         const float zc = inside && (!mask || mask[c]) ? (float)zrow[c] : NEG_INF;
         if (mask) z.mask(mask, h.width, pieces);
@@ -1220,7 +1227,7 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                     inv_r = 1.f / sr;
                     mine[1] += u * inv_r + logf(s * inv_r);
                 }
-                const int c = act[h.slot[d]] - h.low[d];
+                const int c = (int)((uint32_t)act[h.slot[d]] - (uint32_t)h.low[d]);
                 const float v = c >= 0 && c < hi - lo ? logit_at(z, mask, lo + c) : NEG_INF;
                 if (v == NEG_INF) mine[3] += 1.f;
                 else mine[0] += (v - m) - log_s;
@@ -1269,7 +1276,7 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                     inv_r = 1.f / sr;
                     kl += u * inv_r + logf(s * inv_r);
                 }
-                const int c = act[h.slot[d]] - h.low[d];
+                const int c = (int)((uint32_t)act[h.slot[d]] - (uint32_t)h.low[d]);
                 const float v = c >= 0 && c < hi - lo ? logit_at(z, mask, lo + c) : NEG_INF;
                 if (v == NEG_INF) possible = false;
                 else logp += (double)(v - m) - (double)log_s;
@@ -1306,13 +1313,13 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
         for (int d = tid; d < h.n; d += G) {
             const int lo = h.off[d], hi = h.off[d + 1];
             if (hi - lo > LANE_HEAD) continue;
-            const int c = act[h.slot[d]] - h.low[d];
+            const int c = (int)((uint32_t)act[h.slot[d]] - (uint32_t)h.low[d]);
             for (int j = lo; j < hi; j++) one(d, j, c);
         }
         for (int d = 0; d < h.n; d++) {
             const int lo = h.off[d], hi = h.off[d + 1];
             if (hi - lo <= LANE_HEAD) continue;
-            const int c = act[h.slot[d]] - h.low[d];
+            const int c = (int)((uint32_t)act[h.slot[d]] - (uint32_t)h.low[d]);
             for (int j = lo + tid; j < hi; j += G) one(d, j, c);
         }
         __syncthreads();
@@ -1447,7 +1454,7 @@ bool take_wide(const Heads& h, int size, bool loss, WideSplit* w)
 {
     if (h.n != 1 || h.width <= NARROW) return false;
     const int pieces = (h.width * size + 15) / 16;
-    w->v = pieces > (loss ? 1024 : 4096) ? 8 : pieces > 64 ? 4 : 1;
+    w->v = loss && pieces > 1024 ? 8 : pieces > 64 ? 4 : 1;
     const int lanes = (pieces + w->v - 1) / w->v;
     if (lanes > (w->v == 8 ? 512 : 1024)) return false;
     w->lanes = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : lanes <= 64 ? 64 : 0;
@@ -1484,8 +1491,7 @@ void launch_sample(const SampleArgs& a, const Heads& h, hipStream_t st)
     if (take_wide(h, sizeof(T), false, &w)) {
         const OneHead o{h.width, h.low[0], h.slot[0], h.act_dim};
         if (w.v == 1) launch_sample_wide<T, 1>(a, o, w, st);
-        else if (w.v == 4) launch_sample_wide<T, 4>(a, o, w, st);
-        else hipLaunchKernelGGL((sample_wide_kernel<T, 8, 0>), dim3(wide_blocks(w, a.rows)), dim3(w.threads), 0, st, a, o);
+        else launch_sample_wide<T, 4>(a, o, w, st);
         return;
     }
     Small s;
@@ -1509,15 +1515,10 @@ template <class T, int CM, bool REF>
 void launch_loss_narrow(const LossArgs& a, const Small& s, unsigned blocks, hipStream_t st)
 {
     const size_t sums = (size_t)s.n * (REF ? 5 : 3) * WAVE * 4;
-    if (a.grad) {
-        const size_t lds = 4 * (sums + (s.unit_grad < 0 ? (WAVE * s.width * sizeof(T) + 15) & ~(size_t)15 : 0));
-        if (lds > 64 * 1024)
-            (void)hipFuncSetAttribute((const void*)loss_narrow_kernel<T, CM, REF, true>,
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        hipLaunchKernelGGL((loss_narrow_kernel<T, CM, REF, true>), dim3(blocks), dim3(256), lds, st, a, s);
-    } else {
-        hipLaunchKernelGGL((loss_narrow_kernel<T, CM, REF, false>), dim3(blocks), dim3(256), 4 * sums, st, a, s);
-    }
+    const size_t tile = a.grad && s.unit_grad < 0 ? (WAVE * s.width * sizeof(T) + 15) & ~(size_t)15 : 0, lds = 4 * (sums + tile);
+    const auto k = a.grad ? loss_narrow_kernel<T, CM, REF, true> : loss_narrow_kernel<T, CM, REF, false>;
+    if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    hipLaunchKernelGGL(k, dim3(blocks), dim3(256), lds, st, a, s);
 }
 
 template <class T, int CM>
@@ -1557,7 +1558,7 @@ unsigned launch_loss(const LossArgs& a, const Heads& h, hipStream_t st)
         return blocks;
     }
     Small s;
-    // LDS for four waves' heads and gradients: two workgroups must fit a CU
+    // LDS for four waves' heads and gradients must fit a CU
     const size_t lds = 4 * (size_t)(h.n * (a.ref ? 5 : 3) * WAVE * 4 + WAVE * h.width * sizeof(T) + 16);
     if (take_small(h, a.rows > 1 ? a.ld : 0, a.rows > 1 ? a.ld_ref : 0, &s) && lds <= 160 * 1024) {
         const unsigned blocks = narrow_blocks(a.rows);

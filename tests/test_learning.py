@@ -62,6 +62,15 @@ def test_heads_refused(kw, word):
         PolicyHeads(**kw)
 
 
+def test_loss_of_actions_far_outside():
+    """Differences of actions and lows past int32 are no choice either."""
+    z = torch.zeros(2, 3)
+    heads = PolicyHeads([3], low=[2 ** 31 - 4])
+    act = torch.tensor([[-2 ** 31], [2 ** 31 - 3]], dtype=torch.int32)
+    want = ref.policy_loss(z, act, torch.ones(2), torch.zeros(2), heads)
+    assert want['logp'][0] == -math.inf and abs(float(want['logp'][1]) + math.log(3)) < 1e-12
+
+
 def _loss_kw(N=4, heads=TEAM):
     return dict(logits=torch.zeros(N, heads.n_choices), actions=torch.zeros(N, heads.act_dim, dtype=torch.int32),
                 advantage=torch.zeros(N), old_logp=torch.zeros(N), heads=heads)
@@ -207,6 +216,7 @@ def test_reference_gradients_against_differences():
 LAYOUTS = {
     'team': TEAM, 'rtt': RTT, 'cross': CROSS, 'one': PolicyHeads([1]), 'two': PolicyHeads([1, 2], slots=[2, 0]),
     'odd': PolicyHeads([7, 1, 31], low=[-3, 5, 0], slots=[3, 0, 1], act_dim=6),
+    'pairs20': PolicyHeads([2] * 20), 'ones48': PolicyHeads([1] * 48),
     'w63': PolicyHeads([63]), 'w64': PolicyHeads([64]), 'w65': PolicyHeads([65]), 'w200': PolicyHeads([129, 71]),
     'w513': PolicyHeads([513]), 'w1031': PolicyHeads([1031]), 'w4100': PolicyHeads([4100]),
     'w40003': PolicyHeads([40003]), 'two_wide': PolicyHeads([5000, 3, 5000]),
@@ -372,6 +382,12 @@ def test_policy_loss_impossible_actions():
     got = learning.policy_loss_grad(*cuda(z, act, adv, torch.zeros(5)), TEAM, choice_mask=mask.cuda(), entropy_coef=0.1)
     assert (got.logp == -math.inf).all().item()
     check_loss(got, want, torch.float32)
+    for sizes in ([3], [100], [3, 100]):                         # differences past int32, in every kernel
+        heads = PolicyHeads(sizes, low=[2 ** 31 - 1 - n for n in sizes])
+        act = torch.tensor([[-2 ** 31] * len(sizes), [2 ** 31 - 2] * len(sizes)], dtype=torch.int32)
+        z = torch.randn(2, sum(sizes), generator=gen(2))
+        want = ref.policy_loss(z, act, torch.ones(2), torch.zeros(2), heads)
+        check_loss(learning.policy_loss_grad(*cuda(z, act, torch.ones(2), torch.zeros(2)), heads), want, torch.float32)
 
 
 @gpu
@@ -384,6 +400,9 @@ def test_policy_loss_lanes_strides_denominator_scale(dtype):
     zs = wide.cuda()[:, 5:5 + Cn]
     ks = torch.cat([k, k], 1).cuda()[:, Cn:]
     actc, advc, oldc, vc, mc = cuda(act, adv, old, valid.bool(), mask.bool())
+    nothing = learning.policy_loss_grad(zs, actc, advc, oldc, heads, valid=vc, choice_mask=mc,
+                                        denominator=torch.tensor(-1.0).cuda())
+    assert nothing.loss.item() == 0.0 and nothing.count.item() == 0.0 and not nothing.grad.any().item()
     for den in (1000.0, torch.tensor(1000.0).cuda()):
         want = ref.policy_loss(z, act, adv, old, heads, k, valid, mask, clip=(0.1, 0.3), kl_coef=0.1, entropy_coef=0.0,
                                denominator=1000.0, scale=4096.0)
