@@ -510,6 +510,32 @@ def test_odd_addresses_and_strides(name, dtype):
 
 
 @gpu
+@pytest.mark.parametrize('sizes', [[5, 5] + [2] * 9, [2] * 30, [100]], ids=['narrow', 'heads', 'wide'])
+def test_float32_log_probabilities_lean_nowhere(sizes):
+    """Float32 errors that point one way add up over heads and rows: the mean
+    error of a log-probability and of the KL is under half a rounding at 1
+    (2^-25) per head.  What may lean: log2(e) and log(2), 1.4e-8 and 3e-9 of the
+    logits' distance from their mean, and 3e-9 of the exponentials."""
+    N, g = 65536, gen(5)
+    heads = PolicyHeads(sizes)
+    z = 1.5 * torch.randn(N, sum(sizes), generator=g)
+    r = z + 0.2 * torch.randn(z.shape, generator=g)
+    acts, lp, kl, first = [], 0., 0., 0
+    for n in sizes:
+        p, q = (t[:, first:first + n].double().log_softmax(1) for t in (z, r))
+        acts.append((p + gumbel(p.shape, g)).argmax(1))
+        lp = lp + p.gather(1, acts[-1][:, None])[:, 0]
+        kl = kl + (q.exp() * (q - p)).sum(1)
+        first += n
+    args = cuda(z, torch.stack(acts, 1).int(), torch.randn(N, generator=g), lp.float())
+    got = learning.policy_loss_grad(*args, heads, ref_logits=r.cuda(), kl_coef=1.0)
+    bound = len(sizes) * 2. ** -25
+    assert abs((got.logp.cpu().double() - lp).mean()) <= bound
+    # (the mean itself is rounded to float32)
+    assert abs(got.stats[1].cpu().double() - kl.mean()) <= bound + 2. ** -24 * kl.mean()
+
+
+@gpu
 def test_masked_by_the_lowest_value():
     """Choices masked by their type's lowest number, as some policies do, with
     a large loss scale: probability 0, gradient 0, nothing infinite."""
