@@ -84,23 +84,20 @@ constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 1/x and the logarithm of sums of exponentials and of their quotients: the
-// hardware's, and for float32 logits a step of Newton's behind it.  The hardware's
-// logarithm cuts off: over 2^20 values from 2^-10 to 2^3 its mean error was -1.6e-7
-// (at most 9.5e-7), and a log-probability of eleven heads was 8e-7 too high in the
-// mean.  log x = l + (x e^-l - 1) takes that to 4e-8, as 2^x errs by 2.6e-8 (root mean
-// square; mean -3e-9); 1/x by 2.8e-8 (mean -6e-9, which a KL of eleven heads shows).
-template <class T>
+// hardware's, and a step of Newton's behind it.  The hardware's logarithm cuts off:
+// over 2^20 values from 2^-10 to 2^3 its mean error was -1.6e-7 (at most 9.5e-7), and
+// a log-probability of eleven heads was 8e-7 too high in the mean.
+// log x = l + (x e^-l - 1) takes that to 4e-8, as 2^x errs by 2.6e-8 (root mean square;
+// mean -3e-9); 1/x by 2.8e-8 (mean -6e-9, which a KL of eleven heads shows).  Twice a
+// head, it costs the narrow rows 2 to 3% (5.2 M rows of 3, 3, 2: 143 to 147 us).
 __device__ __forceinline__ float rcp_of(float x)
 {
     const float r = __builtin_amdgcn_rcpf(x);
-    if constexpr (sizeof(T) != 4) return r;
     return fmaf(fmaf(-x, r, 1.f), r, r);
 }
-template <class T>
 __device__ __forceinline__ float log_of(float x)
 {
     const float l = __builtin_amdgcn_logf(x);
-    if constexpr (sizeof(T) != 4) return l * LN2;
     return fmaf(l, LN2, fmaf(x, exp2_of(-l), -1.f));
 }
 
@@ -156,7 +153,7 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
                     s += e;
                     t += e * (v - m);
                 }
-                const float log_s = log_of<float>(s);
+                const float log_s = log_of(s);
                 logp += (at - m) - log_s;
                 entropy += log_s - t / s;
             }
@@ -205,7 +202,7 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
             }
             s = grp.sum(s);
             t = grp.sum(t);
-            const float log_s = log_of<float>(s);
+            const float log_s = log_of(s);
             row_logp += (double)(logit_at(z, mask, bi) - m) - (double)log_s;
             row_entropy += log_s - t / s;
             if (tid == 0) act[h.slot[d]] = h.low[d] + (bi - lo);
@@ -538,9 +535,9 @@ __global__ __launch_bounds__(256) void sample_narrow_kernel(SampleArgs a, Small 
             at = better ? v[j] : at;
             if (bit(b.ends, j)) {
                 const bool some = sum != 0.f;
-                const float log_s = some ? log_of<T>(sum) : 0.f;
+                const float log_s = some ? log_of(sum) : 0.f;
                 logp += some ? (double)at - (double)log_s : 0.;
-                entropy += some ? log_s - t * rcp_of<T>(sum) : 0.f;
+                entropy += some ? log_s - t * rcp_of(sum) : 0.f;
                 if (there) acts[act + h.slot[d]] = h.low[d] + (choice < 0 ? 0 : choice - first);
                 sum = t = 0.f;
                 best = NEG_INF;
@@ -749,7 +746,7 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
         for (int d = 0; d < h.n; d++, plane += PLANES * WAVE) {
             const float sd = plane[P_S * WAVE], atd = plane[P_AT * WAVE];
             const bool some = sd != 0.f;
-            const float inv = some ? rcp_of<T>(sd) : 0.f, log_s = some ? log_of<T>(sd) : 0.f, ts = plane[P_T * WAVE] * inv;
+            const float inv = some ? rcp_of(sd) : 0.f, log_s = some ? log_of(sd) : 0.f, ts = plane[P_T * WAVE] * inv;
             const Picks of = ((Picks)~(Picks)0 >> (8 * (int)sizeof(Picks) - h.size[d])) << h.first[d];
             const bool found = (picks & of) != 0 && atd > -1e38f;
             entropy += log_s - ts * LN2;
@@ -758,8 +755,8 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
             if constexpr (REF) {
                 const float srd = plane[P_SR * WAVE];
                 const bool some_ref = some && srd != 0.f;
-                const float inv_r = some_ref ? rcp_of<T>(srd) : 0.f;
-                kl += some_ref ? plane[P_U * WAVE] * inv_r * LN2 + log_of<T>(sd * inv_r) : 0.f;
+                const float inv_r = some_ref ? rcp_of(srd) : 0.f;
+                kl += some_ref ? plane[P_U * WAVE] * inv_r * LN2 + log_of(sd * inv_r) : 0.f;
                 if (GRAD) plane[P_SR * WAVE] = inv_r;
             }
             if (GRAD) {
@@ -1054,10 +1051,10 @@ __global__ __launch_bounds__(L ? 256 : 1024) void sample_wide_kernel(SampleArgs 
         const int c = choice == INT32_MAX ? 0 : choice;
         int32_t* act = a.actions + row * h.act_dim;
         for (int i = 0; i < h.act_dim; i++) act[i] = i == h.slot ? h.low + c : 0;
-        const float log_s = some ? log_of<T>(q[0]) : 0.f;
+        const float log_s = some ? log_of(q[0]) : 0.f;
         if (a.logp)
             a.logp[row] = some ? (float)((double)((float)((const T*)a.logits)[row * a.ld + c] - top) - (double)log_s) : 0.f;
-        if (a.entropy) a.entropy[row] = some ? log_s - q[1] * rcp_of<T>(q[0]) : 0.f;
+        if (a.entropy) a.entropy[row] = some ? log_s - q[1] * rcp_of(q[0]) : 0.f;
     }
 }
 
@@ -1121,9 +1118,9 @@ __global__ __launch_bounds__(L ? 256 : V == 8 ? 512 : 1024) void loss_wide_kerne
         else sum(std::false_type{});
         over_group<L, REF ? 4 : 2>(q, box, [](float p, float o) { return p + o; });
         const bool some = q[0] != 0.f, some_ref = REF && some && q[2] != 0.f;
-        const float inv = some ? rcp_of<T>(q[0]) : 0.f, log_s = some ? log_of<T>(q[0]) : 0.f, ts = q[1] * inv;
-        const float inv_r = some_ref ? rcp_of<T>(q[2]) : 0.f;
-        const float kl = some_ref ? q[3] * inv_r * LN2 + log_of<T>(q[0] * inv_r) : 0.f;
+        const float inv = some ? rcp_of(q[0]) : 0.f, log_s = some ? log_of(q[0]) : 0.f, ts = q[1] * inv;
+        const float inv_r = some_ref ? rcp_of(q[2]) : 0.f;
+        const float kl = some_ref ? q[3] * inv_r * LN2 + log_of(q[0] * inv_r) : 0.f;
         const bool found = some && zc != NEG_INF;
         // as the sums have it: with the rounding of top
         const float xc = fabsf(top) < 1e30f && zc > -1e30f ? fmaf(zc, LOG2E, -top * LOG2E) : (zc - top) * LOG2E;
@@ -1233,13 +1230,13 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                         u += er * (w - (v - m));
                     }
                 }
-                log_s = log_of<float>(s);
+                log_s = log_of(s);
                 inv = 1.f / s;
                 ent = log_s - t * inv;
                 mine[2] += ent;
                 if (zr && mr != NEG_INF) {
                     inv_r = 1.f / sr;
-                    mine[1] += u * inv_r + log_of<float>(s * inv_r);
+                    mine[1] += u * inv_r + log_of(s * inv_r);
                 }
                 const int c = (int)((uint32_t)act[h.slot[d]] - (uint32_t)h.low[d]);
                 const float v = c >= 0 && c < hi - lo ? logit_at(z, mask, lo + c) : NEG_INF;
@@ -1280,7 +1277,7 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                 }
                 s = grp.sum(s);
                 t = grp.sum(t);
-                log_s = log_of<float>(s);
+                log_s = log_of(s);
                 inv = 1.f / s;
                 ent = log_s - t * inv;
                 entropy += ent;
@@ -1288,7 +1285,7 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                     sr = grp.sum(sr);
                     u = grp.sum(u);
                     inv_r = 1.f / sr;
-                    kl += u * inv_r + log_of<float>(s * inv_r);
+                    kl += u * inv_r + log_of(s * inv_r);
                 }
                 const int c = (int)((uint32_t)act[h.slot[d]] - (uint32_t)h.low[d]);
                 const float v = c >= 0 && c < hi - lo ? logit_at(z, mask, lo + c) : NEG_INF;

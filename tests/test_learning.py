@@ -510,16 +510,17 @@ def test_odd_addresses_and_strides(name, dtype):
 
 
 @gpu
+@pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('sizes', [[5, 5] + [2] * 9, [2] * 30, [100]], ids=['narrow', 'heads', 'wide'])
-def test_float32_log_probabilities_lean_nowhere(sizes):
-    """Float32 errors that point one way add up over heads and rows: the mean
+def test_log_probabilities_lean_nowhere(sizes, dtype):
+    """Errors that point one way add up over heads and rows: the mean
     error of a log-probability and of the KL is under half a rounding at 1
     (2^-25) per head.  What may lean: log2(e) and log(2), 1.4e-8 and 3e-9 of the
     logits' distance from their mean, and 3e-9 of the exponentials."""
     N, g = 65536, gen(5)
     heads = PolicyHeads(sizes)
-    z = 1.5 * torch.randn(N, sum(sizes), generator=g)
-    r = z + 0.2 * torch.randn(z.shape, generator=g)
+    z = (1.5 * torch.randn(N, sum(sizes), generator=g)).to(dtype)
+    r = (z + 0.2 * torch.randn(z.shape, generator=g)).to(dtype)
     acts, lp, kl, first = [], 0., 0., 0
     for n in sizes:
         p, q = (t[:, first:first + n].double().log_softmax(1) for t in (z, r))
