@@ -29,6 +29,14 @@ struct RecurArgs {
 // Where channels and waves do not fill the device, the steps are cut into
 // chunks too: a first launch makes every chunk's map (reading gates and
 // values), a second composes the maps before its own and walks.
+//
+// Memory bounds long slabs, launches and round trips short ones:
+//   20 steps of 1048576 channels bf16, a cut a step: 41 us forward (143 MB, 3.5
+//     TB/s) and 48 us backward (227 MB, 4.7 TB/s), by pairs (below);
+//   65537 steps of 96 channels f32, a gate a step: maps 12 and 12 us, walks 19 and
+//     28 us, parts of the gates' sums 4 us, where 127 MB would take 24 us: a
+//     chunk's 8 waves wait for each other's maps, and for those of the chunks before;
+//   one step of 262144 channels bf16: 7.0 us, a launch and one round trip.
 
 struct Map { float a, b; };
 
@@ -554,7 +562,9 @@ __device__ __forceinline__ uint32_t load_steps(const AdvArgs& a, int64_t n, int6
 }
 
 // The recurrence from the last step to the first, split as the gradient's
-// (MAPS: the chunks' maps only).
+// (MAPS: the chunks' maps only).  Memory bounds it: 100 steps of 4096 envs of 64
+// lanes, float64 rewards and float32 values: 127 us, 578 MB at 4.6 TB/s (a copy:
+// 5.2).  5003 steps of 15 lanes: 7.8 us of maps and 12 us of walk, both latency.
 template <class TR, class TV, int NW, int CW, bool MAPS>
 __global__ __launch_bounds__(64 * NW * CW) void advantages_kernel(AdvArgs a, Chunks s)
 {
@@ -657,7 +667,7 @@ void launch_advantages(const AdvArgs& a, void* workspace, hipStream_t st)
 bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
 // Whether 16-bit channels go in pairs: where channels alone fill the device
-// (20 steps of 1048576 channels bf16, forward and backward: 92 us, 135 us one
+// (20 steps of 1048576 channels bf16, forward and backward: 89 us, 135 us one
 // a lane), pairs share what is shared and nothing lies at odd places.
 template <class T, class TG>
 bool take_pairs(const RecurArgs& a, RecurArgs* b)
