@@ -35,7 +35,9 @@ struct Heads {
     int32_t off[GW_MAX_HEADS + 1];
     int32_t low[GW_MAX_HEADS];
     int16_t slot[GW_MAX_HEADS];
+    int16_t large[GW_MAX_HEADS], n_large;       // the heads of more than LANE_HEAD choices
 };
+constexpr int LANE_HEAD = 16;
 
 struct SampleArgs {
     const void* logits; int64_t ld, rows;
@@ -121,11 +123,39 @@ __device__ __forceinline__ float logit_at(const T* row, const uint8_t* mask, int
 // threads.  Heads of up to LANE_HEAD choices are walked by one lane each (the
 // cells of an attack window are dozens of heads of a few choices), larger ones
 // by the whole group, their choices strided over it.  Right for every layout.
-// Latency and idle lanes bound it, not the memory: 65536 rows of 51 heads (214
-// choices bf16) are drawn in 171 us, their loss and gradient take 358 us (a wave
-// a row; the bytes alone take 19 us in either).  G grows with the row, so that a
-// large head's walk stays short.
-constexpr int LANE_HEAD = 16;
+// G grows with the row, so that a large head's walk stays short.  Where a wave
+// takes a row (below STAGED_ROW choices) the row is copied to LDS first, and the
+// gradient leaves from there: the walks over heads would read the memory in pieces of
+// a head, one after the other.  65536 rows of 51 heads (214 choices bf16): drawn in
+// 77 us (171 without), loss and gradient with ref 174 us (358), where the bytes take
+// 19 us in either; the heads' walks, a few choices each, one after another, bound it.
+constexpr int STAGED_ROW = 1024;
+
+// a row to LDS as float, its loads side by side and four in flight; masked choices as -inf
+template <class T, int G>
+__device__ __forceinline__ void stage_row(const T* row, const uint8_t* mask, int width, float* to)
+{
+    for (int j = threadIdx.x; j < width; j += 4 * G) {
+        T v[4];
+        uint8_t m[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int at = j + k * G < width ? j + k * G : width - 1;
+            v[k] = row[at];
+            m[k] = mask ? mask[at] : 1;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (j + k * G < width) to[j + k * G] = m[k] ? (float)v[k] : NEG_INF;
+    }
+}
+
+// A lane's first head, read once: what stands at a lane's own place in the
+// arguments is a load from memory.
+struct OwnHead {
+    int lo, hi, slot, low;
+    __device__ __forceinline__ OwnHead(const Heads& h, int d) : lo(h.off[d]), hi(h.off[d + 1]), slot(h.slot[d]), low(h.low[d]) {}
+};
 
 template <class T, int G>
 __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
@@ -133,13 +163,25 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
     __shared__ float box[G / WAVE];
     __shared__ float best_s[G / WAVE];
     __shared__ int best_i[G / WAVE];
+    extern __shared__ float lds_row[];          // STAGED: the row, its noise
+    constexpr bool STAGED = G == WAVE;
     Group<G> grp{box};
     const int tid = threadIdx.x;
+    const OwnHead own(h, tid < h.n ? tid : 0);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* z = (const T*)a.logits + row * a.ld;
         const float* noise = a.noise ? a.noise + row * h.width : nullptr;
         const uint8_t* mask = a.mask ? a.mask + (row % a.mask_rows) * h.width : nullptr;
         int32_t* act = a.actions + row * h.act_dim;
+        if constexpr (STAGED) {
+            stage_row<T, G>(z, mask, h.width, lds_row);
+            if (noise) stage_row<float, G>(noise, nullptr, h.width, lds_row + h.width);
+            __syncthreads();
+        }
+        const auto logit = [&](int j) __attribute__((always_inline)) { return STAGED ? lds_row[j] : logit_at(z, mask, j); };
+        const auto score = [&](int j, float v) __attribute__((always_inline)) {
+            return noise ? v + (STAGED ? lds_row[h.width + j] : noise[j]) : v;
+        };
         if (h.n < h.act_dim)
             for (int c = tid; c < h.act_dim; c += G) {
                 bool owned = false;
@@ -148,20 +190,21 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
             }
         float logp = 0.f, entropy = 0.f;                 // of this lane's heads; the group's in lane 0
         for (int d = tid; d < h.n; d += G) {
-            const int lo = h.off[d], hi = h.off[d + 1];
+            const OwnHead mine = d == tid ? own : OwnHead(h, d);
+            const int lo = mine.lo, hi = mine.hi;
             if (hi - lo > LANE_HEAD) continue;
             float m = NEG_INF, bs = NEG_INF, at = 0.f, s = 0.f, t = 0.f;
             int bi = -1;
             for (int j = lo; j < hi; j++) {
-                const float v = logit_at(z, mask, j);
+                const float v = logit(j);
                 if (v == NEG_INF) continue;
                 m = max_nan(m, v);
-                const float sc = noise ? v + noise[j] : v;
+                const float sc = score(j, v);
                 if (sc > bs || (bi < 0 && sc == bs)) { bs = sc; bi = j; at = v; }
             }
             if (m != NEG_INF) {
                 for (int j = lo; j < hi; j++) {
-                    const float v = logit_at(z, mask, j);
+                    const float v = logit(j);
                     if (v == NEG_INF) continue;
                     const float e = expf(v - m);
                     s += e;
@@ -171,20 +214,19 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
                 logp += (at - m) - log_s;
                 entropy += log_s - t / s;
             }
-            act[h.slot[d]] = h.low[d] + (bi < 0 ? 0 : bi - lo);
+            act[mine.slot] = mine.low + (bi < 0 ? 0 : bi - lo);
         }
         double row_logp = 0.;
         float row_entropy = 0.f;
-        for (int d = 0; d < h.n; d++) {
-            const int lo = h.off[d], hi = h.off[d + 1];
-            if (hi - lo <= LANE_HEAD) continue;
+        for (int i = 0; i < h.n_large; i++) {
+            const int d = h.large[i], lo = h.off[d], hi = h.off[d + 1];
             float m = NEG_INF, bs = NEG_INF;
             int bi = INT32_MAX;
             for (int j = lo + tid; j < hi; j += G) {
-                const float v = logit_at(z, mask, j);
+                const float v = logit(j);
                 if (v == NEG_INF) continue;
                 m = max_nan(m, v);
-                const float s = noise ? v + noise[j] : v;
+                const float s = score(j, v);
                 if (s > bs || (s == bs && j < bi)) { bs = s; bi = j; }
             }
             m = grp.max(m);
@@ -208,7 +250,7 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
             if (bi == INT32_MAX) bi = lo;                // every score NaN
             float s = 0.f, t = 0.f;
             for (int j = lo + tid; j < hi; j += G) {
-                const float v = logit_at(z, mask, j);
+                const float v = logit(j);
                 if (v == NEG_INF) continue;
                 const float e = expf(v - m);
                 s += e;
@@ -217,7 +259,7 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
             s = grp.sum(s);
             t = grp.sum(t);
             const float log_s = log_of(s);
-            row_logp += (double)(logit_at(z, mask, bi) - m) - (double)log_s;
+            row_logp += (double)(logit(bi) - m) - (double)log_s;
             row_entropy += log_s - t / s;
             if (tid == 0) act[h.slot[d]] = h.low[d] + (bi - lo);
         }
@@ -227,6 +269,7 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
             if (a.logp) a.logp[row] = (float)(row_logp + (double)logp);
             if (a.entropy) a.entropy[row] = row_entropy + entropy;
         }
+        if constexpr (STAGED) __syncthreads();           // the next row goes where this one is
     }
 }
 
@@ -1212,10 +1255,13 @@ template <class T, int G>
 __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
 {
     __shared__ float box[G / WAVE];
-    __shared__ float hm[GW_MAX_HEADS], hls[GW_MAX_HEADS], hinv[GW_MAX_HEADS], hh[GW_MAX_HEADS],
-        hrm[GW_MAX_HEADS], hrinv[GW_MAX_HEADS];
+    extern __shared__ float lds_row[];          // six numbers a head; STAGED: the row (then its gradient), ref's
+    constexpr bool STAGED = G == WAVE;
+    float *hm = lds_row, *hls = hm + h.n, *hinv = hls + h.n, *hh = hinv + h.n, *hrm = hh + h.n, *hrinv = hrm + h.n;
+    float *lz = hrinv + h.n, *lr = lz + h.width;
     Group<G> grp{box};
     const int tid = threadIdx.x;
+    const OwnHead own(h, tid < h.n ? tid : 0);
     double sums[N_SUMS] = {0., 0., 0., 0., 0.};
     float step = 0.f;
     if (a.grad) step = a.scale * (a.upstream ? *a.upstream : 1.f) * inverse_rows(a);
@@ -1231,28 +1277,36 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
         const T* zr = a.ref ? (const T*)a.ref + row * a.ld_ref : nullptr;
         const uint8_t* mask = a.mask ? a.mask + (row % a.mask_rows) * h.width : nullptr;
         const int32_t* act = a.actions + row * h.act_dim;
+        if constexpr (STAGED) {
+            stage_row<T, G>(z, mask, h.width, lz);
+            if (zr) stage_row<T, G>(zr, nullptr, h.width, lr);
+            __syncthreads();
+        }
+        const auto logit = [&](int j) __attribute__((always_inline)) { return STAGED ? lz[j] : logit_at(z, mask, j); };
+        const auto refs = [&](int j) __attribute__((always_inline)) { return STAGED ? lr[j] : (float)zr[j]; };
         // this lane's heads: their parts of L, KL, H, and how many actions were not possible
         float mine[4] = {0.f, 0.f, 0.f, 0.f};
         for (int d = tid; d < h.n; d += G) {
-            const int lo = h.off[d], hi = h.off[d + 1];
+            const OwnHead at = d == tid ? own : OwnHead(h, d);
+            const int lo = at.lo, hi = at.hi;
             if (hi - lo > LANE_HEAD) continue;
             float m = NEG_INF, mr = NEG_INF, s = 0.f, t = 0.f, sr = 0.f, u = 0.f;
             for (int j = lo; j < hi; j++) {
-                const float v = logit_at(z, mask, j);
+                const float v = logit(j);
                 if (v == NEG_INF) continue;
                 m = max_nan(m, v);
-                if (zr) mr = max_nan(mr, (float)zr[j]);
+                if (zr) mr = max_nan(mr, refs(j));
             }
             float log_s = 0.f, inv = 0.f, ent = 0.f, inv_r = 0.f;
             if (m != NEG_INF) {
                 for (int j = lo; j < hi; j++) {
-                    const float v = logit_at(z, mask, j);
+                    const float v = logit(j);
                     if (v == NEG_INF) continue;
                     const float e = expf(v - m);
                     s += e;
                     t += e * (v - m);
-                    if (zr && (float)zr[j] != NEG_INF) {
-                        const float w = (float)zr[j] - mr, er = expf(w);
+                    if (zr && refs(j) != NEG_INF) {
+                        const float w = refs(j) - mr, er = expf(w);
                         sr += er;
                         u += er * (w - (v - m));
                     }
@@ -1265,8 +1319,8 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                     inv_r = 1.f / sr;
                     mine[1] += u * inv_r + log_of(s * inv_r);
                 }
-                const int c = (int)((uint32_t)act[h.slot[d]] - (uint32_t)h.low[d]);
-                const float v = c >= 0 && c < hi - lo ? logit_at(z, mask, lo + c) : NEG_INF;
+                const int c = (int)((uint32_t)act[at.slot] - (uint32_t)at.low);
+                const float v = c >= 0 && c < hi - lo ? logit(lo + c) : NEG_INF;
                 if (v == NEG_INF) mine[3] += 1.f;
                 else mine[0] += (v - m) - log_s;
             }
@@ -1275,15 +1329,14 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
         float kl = 0.f, entropy = 0.f;
         double logp = 0.;
         bool possible = true;
-        for (int d = 0; d < h.n; d++) {
-            const int lo = h.off[d], hi = h.off[d + 1];
-            if (hi - lo <= LANE_HEAD) continue;
+        for (int i = 0; i < h.n_large; i++) {
+            const int d = h.large[i], lo = h.off[d], hi = h.off[d + 1];
             float m = NEG_INF, mr = NEG_INF;
             for (int j = lo + tid; j < hi; j += G) {
-                const float v = logit_at(z, mask, j);
+                const float v = logit(j);
                 if (v == NEG_INF) continue;
                 m = max_nan(m, v);
-                if (zr) mr = max_nan(mr, (float)zr[j]);
+                if (zr) mr = max_nan(mr, refs(j));
             }
             m = grp.max(m);
             if (zr) mr = grp.max(mr);
@@ -1291,13 +1344,13 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
             if (m != NEG_INF) {
                 float s = 0.f, t = 0.f, sr = 0.f, u = 0.f;
                 for (int j = lo + tid; j < hi; j += G) {
-                    const float v = logit_at(z, mask, j);
+                    const float v = logit(j);
                     if (v == NEG_INF) continue;
                     const float e = expf(v - m);
                     s += e;
                     t += e * (v - m);
-                    if (zr && (float)zr[j] != NEG_INF) {
-                        const float w = (float)zr[j] - mr, er = expf(w);
+                    if (zr && refs(j) != NEG_INF) {
+                        const float w = refs(j) - mr, er = expf(w);
                         sr += er;
                         u += er * (w - (v - m));
                     }
@@ -1315,7 +1368,7 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                     kl += u * inv_r + log_of(s * inv_r);
                 }
                 const int c = (int)((uint32_t)act[h.slot[d]] - (uint32_t)h.low[d]);
-                const float v = c >= 0 && c < hi - lo ? logit_at(z, mask, lo + c) : NEG_INF;
+                const float v = c >= 0 && c < hi - lo ? logit(lo + c) : NEG_INF;
                 if (v == NEG_INF) possible = false;
                 else logp += (double)(v - m) - (double)log_s;
             }
@@ -1337,28 +1390,33 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
             continue;
         }
         __syncthreads();
-        const auto one = [&](int d, int j, int c) __attribute__((always_inline)) {
-            const float v = logit_at(z, mask, j);
+        const auto one = [&](int d, int lo, int j, int c) __attribute__((always_inline)) {
+            const float v = logit(j);
             float gj = 0.f;
             if (v != NEG_INF) {
                 const float x = v - hm[d], p = expf(x) * hinv[d];
                 // d(-surrogate) pull (1[chosen] - p), KL p - q, entropy p (log p + H)
-                gj = r.pull * ((j - h.off[d] == c ? 1.f : 0.f) - p) + a.entropy * p * (x - hls[d] + hh[d]);
-                if (hrinv[d] != 0.f) gj += a.kl * (p - expf((float)zr[j] - hrm[d]) * hrinv[d]);
+                gj = r.pull * ((j - lo == c ? 1.f : 0.f) - p) + a.entropy * p * (x - hls[d] + hh[d]);
+                if (hrinv[d] != 0.f) gj += a.kl * (p - expf(refs(j) - hrm[d]) * hrinv[d]);
             }
-            g[j] = (T)(gj * step);
+            if constexpr (STAGED) lz[j] = gj * step;
+            else g[j] = (T)(gj * step);
         };
         for (int d = tid; d < h.n; d += G) {
-            const int lo = h.off[d], hi = h.off[d + 1];
+            const OwnHead at = d == tid ? own : OwnHead(h, d);
+            const int lo = at.lo, hi = at.hi;
             if (hi - lo > LANE_HEAD) continue;
-            const int c = (int)((uint32_t)act[h.slot[d]] - (uint32_t)h.low[d]);
-            for (int j = lo; j < hi; j++) one(d, j, c);
+            const int c = (int)((uint32_t)act[at.slot] - (uint32_t)at.low);
+            for (int j = lo; j < hi; j++) one(d, lo, j, c);
         }
-        for (int d = 0; d < h.n; d++) {
-            const int lo = h.off[d], hi = h.off[d + 1];
-            if (hi - lo <= LANE_HEAD) continue;
+        for (int i = 0; i < h.n_large; i++) {
+            const int d = h.large[i], lo = h.off[d], hi = h.off[d + 1];
             const int c = (int)((uint32_t)act[h.slot[d]] - (uint32_t)h.low[d]);
-            for (int j = lo + tid; j < hi; j += G) one(d, j, c);
+            for (int j = lo + tid; j < hi; j += G) one(d, lo, j, c);
+        }
+        if constexpr (STAGED) {
+            __syncthreads();
+            for (int j = tid; j < h.width; j += G) g[j] = (T)lz[j];
         }
         __syncthreads();
     }
@@ -1425,6 +1483,7 @@ gw_status take_heads(const gw_policy_heads* p, Heads* h)
     LEARN_NEED(p->act_dim >= 1 && p->act_dim <= 32767, "act_dim %d outside 1..32767", p->act_dim);
     h->n = p->n_heads;
     h->act_dim = p->act_dim;
+    h->n_large = 0;
     int64_t w = 0;
     for (int d = 0; d < p->n_heads; d++) {
         LEARN_NEED(p->sizes[d] >= 1, "head %d has %d choices", d, p->sizes[d]);
@@ -1434,6 +1493,7 @@ gw_status take_heads(const gw_policy_heads* p, Heads* h)
         h->off[d] = (int32_t)w;
         h->low[d] = p->low[d];
         h->slot[d] = (int16_t)p->slots[d];
+        if (p->sizes[d] > LANE_HEAD) h->large[h->n_large++] = (int16_t)d;
         w += p->sizes[d];
         LEARN_NEED(w <= (1 << 30), "more than 2^30 choices");
     }
@@ -1548,8 +1608,8 @@ void launch_sample(const SampleArgs& a, const Heads& h, hipStream_t st)
     }
     const dim3 grid((unsigned)blocks_for(a.rows));
     if (h.width >= 8192) hipLaunchKernelGGL((sample_rows_kernel<T, 1024>), grid, dim3(1024), 0, st, a, h);
-    else if (h.width >= 1024) hipLaunchKernelGGL((sample_rows_kernel<T, 256>), grid, dim3(256), 0, st, a, h);
-    else hipLaunchKernelGGL((sample_rows_kernel<T, 64>), grid, dim3(64), 0, st, a, h);
+    else if (h.width >= STAGED_ROW) hipLaunchKernelGGL((sample_rows_kernel<T, 256>), grid, dim3(256), 0, st, a, h);
+    else hipLaunchKernelGGL((sample_rows_kernel<T, 64>), grid, dim3(64), (a.noise ? 2 : 1) * h.width * 4, st, a, h);
 }
 
 template <class T, int CM, bool REF>
@@ -1616,9 +1676,10 @@ unsigned launch_loss(const LossArgs& a, const Heads& h, hipStream_t st)
         return blocks;
     }
     const unsigned blocks = (unsigned)blocks_for(a.rows);
-    if (h.width >= 8192) hipLaunchKernelGGL((loss_rows_kernel<T, 1024>), dim3(blocks), dim3(1024), 0, st, a, h);
-    else if (h.width >= 1024) hipLaunchKernelGGL((loss_rows_kernel<T, 256>), dim3(blocks), dim3(256), 0, st, a, h);
-    else hipLaunchKernelGGL((loss_rows_kernel<T, 64>), dim3(blocks), dim3(64), 0, st, a, h);
+    const unsigned stats = 6 * h.n * 4, staged = stats + (a.ref ? 2 : 1) * h.width * 4;
+    if (h.width >= 8192) hipLaunchKernelGGL((loss_rows_kernel<T, 1024>), dim3(blocks), dim3(1024), stats, st, a, h);
+    else if (h.width >= STAGED_ROW) hipLaunchKernelGGL((loss_rows_kernel<T, 256>), dim3(blocks), dim3(256), stats, st, a, h);
+    else hipLaunchKernelGGL((loss_rows_kernel<T, 64>), dim3(blocks), dim3(64), staged, st, a, h);
     return blocks;
 }
 
