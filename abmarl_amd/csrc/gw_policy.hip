@@ -1546,8 +1546,10 @@ void launch_sample_narrow(const SampleArgs& a, const Small& s, hipStream_t st)
 }
 
 // How a wide head's rows are shared out, or false where registers do not hold
-// them: pieces of 16 bytes, one or (from 65 pieces on) four a lane; fewer than a
-// wave's lanes a row where the row has fewer pieces.  Above 1024 pieces the loss
+// them: pieces of 16 bytes, one or (from 17 pieces on) four a lane; fewer than a
+// wave's lanes a row where the row has fewer pieces.  Four rows' sums then cross a
+// wave's lanes in one (65536 rows of 300 bf16, loss and gradient with ref: 64 us, 94
+// us with one piece a lane; of 65 f32, 17 pieces: 30 and 38).  Above 1024 pieces the loss
 // takes eight a lane: fewer waves a row hold fewer copies of what is not the
 // row, so three rows fit a CU in place of two (4099 x 12800 bf16: 119 us, 130 us
 // with four; drawing 1024 of them f16, one row and its noise, takes 27 us with eight
@@ -1558,7 +1560,7 @@ bool take_wide(const Heads& h, int size, bool loss, WideSplit* w)
 {
     if (h.n != 1 || h.width <= NARROW) return false;
     const int pieces = (h.width * size + 15) / 16;
-    w->v = loss && pieces > 1024 ? 8 : pieces > 64 ? 4 : 1;
+    w->v = loss && pieces > 1024 ? 8 : pieces > 16 ? 4 : 1;
     const int lanes = (pieces + w->v - 1) / w->v;
     if (lanes > (w->v == 8 ? 512 : 1024)) return false;
     w->lanes = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : lanes <= 64 ? 64 : 0;
@@ -1578,14 +1580,13 @@ template <class T, int V>
 void launch_sample_wide(const SampleArgs& a, const OneHead& o, const WideSplit& w, hipStream_t st)
 {
     const dim3 grid(wide_blocks(w, a.rows)), block(w.threads);
-    if constexpr (V == 1) {
-        if (w.lanes == 8) hipLaunchKernelGGL((sample_wide_kernel<T, V, 8>), grid, block, 0, st, a, o);
-        if (w.lanes == 16) hipLaunchKernelGGL((sample_wide_kernel<T, V, 16>), grid, block, 0, st, a, o);
-    }
-    if (w.lanes == 32) hipLaunchKernelGGL((sample_wide_kernel<T, V, 32>), grid, block, 0, st, a, o);
-    if (w.lanes == 64) hipLaunchKernelGGL((sample_wide_kernel<T, V, 64>), grid, block, 0, st, a, o);
-    if constexpr (V > 1)
+    if (w.lanes == 8) hipLaunchKernelGGL((sample_wide_kernel<T, V, 8>), grid, block, 0, st, a, o);
+    if (w.lanes == 16) hipLaunchKernelGGL((sample_wide_kernel<T, V, 16>), grid, block, 0, st, a, o);
+    if constexpr (V > 1) {
+        if (w.lanes == 32) hipLaunchKernelGGL((sample_wide_kernel<T, V, 32>), grid, block, 0, st, a, o);
+        if (w.lanes == 64) hipLaunchKernelGGL((sample_wide_kernel<T, V, 64>), grid, block, 0, st, a, o);
         if (w.lanes == 0) hipLaunchKernelGGL((sample_wide_kernel<T, V, 0>), grid, block, 0, st, a, o);
+    }
 }
 
 template <class T>
@@ -1654,10 +1655,10 @@ unsigned launch_loss(const LossArgs& a, const Heads& h, hipStream_t st)
         const unsigned blocks = wide_blocks(w, a.rows);
         if (w.v == 1) {
             if (w.lanes == 8) launch_loss_wide<T, 1, 8>(a, o, blocks, w.threads, st);
-            else if (w.lanes == 16) launch_loss_wide<T, 1, 16>(a, o, blocks, w.threads, st);
-            else if (w.lanes == 32) launch_loss_wide<T, 1, 32>(a, o, blocks, w.threads, st);
-            else launch_loss_wide<T, 1, 64>(a, o, blocks, w.threads, st);
+            else launch_loss_wide<T, 1, 16>(a, o, blocks, w.threads, st);
         } else if (w.v == 8) launch_loss_wide<T, 8, 0>(a, o, blocks, w.threads, st);
+        else if (w.lanes == 8) launch_loss_wide<T, 4, 8>(a, o, blocks, w.threads, st);
+        else if (w.lanes == 16) launch_loss_wide<T, 4, 16>(a, o, blocks, w.threads, st);
         else if (w.lanes == 32) launch_loss_wide<T, 4, 32>(a, o, blocks, w.threads, st);
         else if (w.lanes == 64) launch_loss_wide<T, 4, 64>(a, o, blocks, w.threads, st);
         else launch_loss_wide<T, 4, 0>(a, o, blocks, w.threads, st);

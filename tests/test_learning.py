@@ -222,6 +222,7 @@ LAYOUTS = {
     'w40003': PolicyHeads([40003]), 'two_wide': PolicyHeads([5000, 3, 5000]),
     'many': PolicyHeads([15, 15] + [2] * 225), 'cells': PolicyHeads([17, 17] + [4] * 49), 'mixed': PolicyHeads([3, 1500, 2, 700]),
     'w19': PolicyHeads([7, 7, 5]), 'w24': PolicyHeads([11, 11, 2]), 'w33': PolicyHeads([15, 15, 3]), 'w47': PolicyHeads([9, 31, 7]),
+    'w129': PolicyHeads([129]), 'w250': PolicyHeads([250]), 'w257': PolicyHeads([257]), 'w300': PolicyHeads([300]),
     'w1023': PolicyHeads([1000, 23]), 'w1024': PolicyHeads([1000, 24]),
 }
 ROWS = {'w513': 9, 'w1031': 5, 'w4100': 3, 'many': 7, 'mixed': 4, 'w200': 13, 'w40003': 2, 'two_wide': 2, 'cells': 11,
