@@ -93,6 +93,12 @@ struct Group {
 };
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+// The largest |top| for which logits become exponents by one fma, z log2(e) -
+// round(top log2(e)).  The rounding shifts all exponents of a row alike, which cancels in
+// what they are used for, as long as all of them are made this way; here it is under 2^-7.
+// (At 1e10 it would be 440, and 2^440 infinite.)  Every float16 is in.
+constexpr float NEAR_TOP = 65536.f;
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 1/x and the logarithm of sums of exponentials and of their quotients: the
@@ -642,7 +648,7 @@ __device__ __forceinline__ bool row_span(const float* v, int width, float& top)
         top = fmaxf(top, v[j]);
         low = fminf(low, j < width ? v[j] : -NEG_INF);
     }
-    return low > top - SPAN && fabsf(top) < 1e30f;
+    return low > top - SPAN && fabsf(top) < NEAR_TOP;
 }
 
 // the same over the choices that exist
@@ -652,7 +658,7 @@ __device__ __forceinline__ bool some_span(const float* v, float top)
     float low = -NEG_INF;
 #pragma unroll
     for (int j = 0; j < CM; j++) low = fminf(low, v[j] == NEG_INF ? -NEG_INF : v[j]);
-    return top == NEG_INF || (low > top - SPAN && fabsf(top) < 1e30f);
+    return top == NEG_INF || (low > top - SPAN && fabsf(top) < NEAR_TOP);
 }
 
 template <int CM, bool ALL>
@@ -900,6 +906,16 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
 // 60 us of it are arithmetic, and three rows a CU leave the loads of a row, which
 // all come first, uncovered in part.  1024 rows f16 drawn with their noise: 24 us, 79 MB
 // at 3.2 TB/s (the bytes: 15 us), by four rows a CU that start together.
+
+// (logit - top) log2(e) of a row, one form for all of its choices: beside a top
+// under NEAR_TOP one fma, else the difference first
+struct Base {
+    float far, shift;
+    __device__ __forceinline__ explicit Base(float top)
+        : far(fabsf(top) < NEAR_TOP ? 0.f : top), shift(fabsf(top) < NEAR_TOP ? -top * LOG2E : 0.f) {}
+    __device__ __forceinline__ float exponent(float z) const { return fmaf(z - far, LOG2E, shift); }
+};
+
 template <class T, int V, int L>
 struct WideRow {
     static constexpr int PER = 16 / sizeof(T), WORD = 4 / sizeof(T);
@@ -987,16 +1003,16 @@ struct WideRow {
                     lo = fminf(lo, get(k, e));
                 }
     }
-    // (logit - top) log2(e).  PLAIN: every choice exists and all are of ordinary
-    // size: one fma; its rounding of `top` is common to all choices and to
-    // their sum, so it cancels
+    // The logit's exponent.  PLAIN: every choice exists and all are of ordinary size,
+    // top too: one fma.  Whether it is PLAIN may differ between the waves of a row
+    // and between the sums and the gradient; the exponent is the same to the bit.
     template <bool PLAIN>
-    __device__ __forceinline__ float less(int k, int e, float top) const
+    __device__ __forceinline__ float less(int k, int e, const Base& b) const
     {
         const float z = get(k, e);
-        if constexpr (PLAIN) return fmaf(z, LOG2E, -top * LOG2E);
+        if constexpr (PLAIN) return fmaf(z, LOG2E, b.shift);
         // a choice 1e30 below the best (masked by its type's lowest value) is as far as any
-        const float x = (z - top) * LOG2E;
+        const float x = b.exponent(z);
         return z == NEG_INF ? NO_CHOICE : x < -1e30f ? -1e30f : x;
     }
     // what was made of the row before is not to be kept beside it: it is made again
@@ -1084,6 +1100,7 @@ __global__ __launch_bounds__(L ? 256 : 1024) void sample_wide_kernel(SampleArgs 
         const bool whole = low > -1e30f;
         over_group<L, 1>(m, box, [](float p, float q) { return fmaxf(p, q); });
         const float top = m[0] == NEG_INF ? 0.f : m[0];
+        const Base base(top);
         float q[2] = {0.f, 0.f};
         const auto sum = [&](auto plain) __attribute__((always_inline)) {
 #pragma unroll
@@ -1091,14 +1108,14 @@ __global__ __launch_bounds__(L ? 256 : 1024) void sample_wide_kernel(SampleArgs 
                 if (k >= pieces) continue;
 #pragma unroll
                 for (int e = 0; e < Row::PER; e++) {
-                    const float x = z.template less<decltype(plain)::value>(k, e, top), ex = exp2_of(x);
+                    const float x = z.template less<decltype(plain)::value>(k, e, base), ex = exp2_of(x);
                     q[0] += ex;
                     q[1] += ex * x;
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        if (__all(whole && fabsf(top) < 1e30f)) sum(std::true_type{});
+        if (__all(whole && fabsf(top) < NEAR_TOP)) sum(std::true_type{});
         else sum(std::false_type{});
         q[1] *= LN2;
         over_group<L, 2>(q, box, [](float p, float r) { return p + r; });
@@ -1124,8 +1141,9 @@ __global__ __launch_bounds__(L ? 256 : 1024) void sample_wide_kernel(SampleArgs 
         int32_t* act = a.actions + row * h.act_dim;
         for (int i = 0; i < h.act_dim; i++) act[i] = i == h.slot ? h.low + c : 0;
         const float log_s = some ? log_of(q[0]) : 0.f;
+        // (of the exponent that the sums have, as the loss makes it)
         if (a.logp)
-            a.logp[row] = some ? (float)((double)((float)((const T*)a.logits)[row * a.ld + c] - top) - (double)log_s) : 0.f;
+            a.logp[row] = some ? (float)((double)(base.exponent((float)((const T*)a.logits)[row * a.ld + c]) * LN2) - (double)log_s) : 0.f;
         if (a.entropy) a.entropy[row] = some ? log_s - q[1] * rcp_of(q[0]) : 0.f;
     }
 }
@@ -1165,8 +1183,9 @@ __global__ __launch_bounds__(L ? 256 : V == 8 ? 512 : 1024) void loss_wide_kerne
         z.forget();
         over_group<L, REF ? 2 : 1>(m, box, [](float p, float o) { return fmaxf(p, o); });
         const float top = m[0] == NEG_INF ? 0.f : m[0], top_r = m[1] == NEG_INF ? 0.f : m[1];
+        const Base base(top), base_r(top_r);
         // (by waves: most rows are plain but for the pieces behind their ends)
-        const bool plain_wave = __all(low > -1e30f && low_r > -1e30f && fabsf(top) < 1e30f && fabsf(top_r) < 1e30f);
+        const bool plain_wave = __all(low > -1e30f && low_r > -1e30f && fabsf(top) < NEAR_TOP && fabsf(top_r) < NEAR_TOP);
         const auto sum = [&](auto plain) __attribute__((always_inline)) {
             constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
@@ -1174,11 +1193,11 @@ __global__ __launch_bounds__(L ? 256 : V == 8 ? 512 : 1024) void loss_wide_kerne
                 if (k >= pieces) continue;
 #pragma unroll
                 for (int e = 0; e < PER; e++) {
-                    const float x = z.template less<PLAIN>(k, e, top), ex = exp2_of(x);
+                    const float x = z.template less<PLAIN>(k, e, base), ex = exp2_of(x);
                     q[0] += ex;
                     q[1] += ex * x;
                     if constexpr (REF) {
-                        const float y = r.template less<PLAIN>(k, e, top_r), ey = exp2_of(y);
+                        const float y = r.template less<PLAIN>(k, e, base_r), ey = exp2_of(y);
                         q[2] += ey;
                         q[3] += ey * (y - x);
                     }
@@ -1194,9 +1213,7 @@ __global__ __launch_bounds__(L ? 256 : V == 8 ? 512 : 1024) void loss_wide_kerne
         const float inv_r = some_ref ? rcp_of(q[2]) : 0.f;
         const float kl = some_ref ? q[3] * inv_r * LN2 + log_of(q[0] * inv_r) : 0.f;
         const bool found = some && zc != NEG_INF;
-        // as the sums have it: with the rounding of top
-        const float xc = fabsf(top) < 1e30f && zc > -1e30f ? fmaf(zc, LOG2E, -top * LOG2E) : (zc - top) * LOG2E;
-        const double logp = found ? (double)(xc * LN2) - (double)log_s : 0.;
+        const double logp = found ? (double)(base.exponent(zc) * LN2) - (double)log_s : 0.;
         const RowLoss got = row_loss(a, a.advantage[row], a.old_logp[row], logp, found || !some, kl, log_s - ts * LN2);
         if (Rows<L>::leader() && mine < a.rows) {
             if (a.logp) a.logp[row] = valid ? got.logp : 0.f;
@@ -1221,9 +1238,9 @@ __global__ __launch_bounds__(L ? 256 : V == 8 ? 512 : 1024) void loss_wide_kerne
                     float g[PER];
 #pragma unroll
                     for (int e = 0; e < PER; e++) {
-                        const float x = z.template less<PLAIN>(k, e, top);
+                        const float x = z.template less<PLAIN>(k, e, base);
                         g[e] = exp2_of(x) * fmaf(a1, x, a0);
-                        if constexpr (REF) g[e] = fmaf(b, exp2_of(r.template less<PLAIN>(k, e, top_r)), g[e]);
+                        if constexpr (REF) g[e] = fmaf(b, exp2_of(r.template less<PLAIN>(k, e, base_r)), g[e]);
                         if (!PLAIN) g[e] = valid && x != NO_CHOICE ? g[e] : 0.f;
                     }
                     if (found && valid && (uint32_t)(c - j) < (uint32_t)PER && c >= own)

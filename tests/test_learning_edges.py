@@ -1,0 +1,96 @@
+"""The policy operators at the ends of their range, against the same 64-bit
+definitions and counted bounds."""
+import math
+
+import pytest
+import torch
+
+from abmarl_amd import learning
+from abmarl_amd.learning import PolicyHeads
+from tests import learning_reference as ref
+from tests.test_learning import DTYPES, LAYOUTS, check_loss, cuda, gen, gumbel
+
+gpu = pytest.mark.gpu
+
+NARROW = ['team', 'rtt', 'odd', 'w47']
+
+
+def offsets(dtype):
+    far = [1e3, 6e4] if dtype == torch.float16 else [1e3, 6e4, 1e6, 1.3e8, 2.6e8, 1e10, 1e20, 1e38]
+    return far + [-v for v in far]
+
+
+def far_inputs(heads, dtype, offset, seed, N, masked):
+    """Rows around `offset` (row 0 equal to it throughout, row 1 around 0), ref
+    logits, masks, actions, advantages and what the actions' log-probabilities
+    were a little before."""
+    g = gen(seed)
+    shape = (N, heads.n_choices)
+    z = offset + 1.7 * torch.randn(shape, generator=g, dtype=torch.float64)
+    z[0] = offset
+    z[1] -= offset
+    z = z.to(dtype)
+    k = (z.double() + 0.3 * torch.randn(shape, generator=g, dtype=torch.float64)).to(dtype)
+    mask = None
+    if masked:
+        mask = (torch.rand(shape, generator=g) < 0.7).to(torch.uint8)
+        mask[:2] = 1
+        z = torch.where(mask == 0, torch.tensor(math.nan, dtype=dtype), z)
+    noise = gumbel(shape, g)
+    act, logp, _, _, _ = ref.sample(z, heads, noise, mask)
+    old = (logp - 0.1 * torch.rand(N, generator=g)).float()      # no ratio at the border of the clipping
+    valid = (torch.rand(N, generator=g) < 0.7).to(torch.uint8)
+    valid[0] = 1
+    return z, k, mask, noise, act, torch.randn(N, generator=g), old, valid
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('masked', [False, True])
+@pytest.mark.parametrize('name', NARROW)
+def test_loss_of_logits_of_any_size(name, masked, dtype):
+    """Only differences of a head's logits count, however large they are."""
+    heads = LAYOUTS[name]
+    kw = dict(kl_coef=0.3, entropy_coef=0.02)
+    for i, offset in enumerate(offsets(dtype)):
+        z, k, mask, _, act, adv, old, valid = far_inputs(heads, dtype, offset, i, 67, masked)
+        for r, v in ((None, valid), (k, None)):
+            want = ref.policy_loss(z, act, adv, old, heads, r, v, mask, **kw)
+            zc, actc, advc, oldc, rc, vc, mc = cuda(z, act, adv, old, r, v, mask)
+            got = learning.policy_loss_grad(zc, actc, advc, oldc, heads, ref_logits=rc, valid=vc, choice_mask=mc, **kw)
+            check_loss(got, want, dtype)
+
+
+WIDE = {'w65': 67, 'w300': 31, 'w513': 9, 'w4100': 5, 'w12801': 5}
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('masked', [False, True])
+@pytest.mark.parametrize('name', list(WIDE))
+def test_wide_rows_of_any_size(name, masked, dtype):
+    """One wide head: the waves and lanes of a row count its differences alike,
+    whether or not a choice of theirs is masked, and a row that is not valid
+    changes nothing for its neighbours; what is drawn has the loss's own log-probability."""
+    heads, N = PolicyHeads([int(name[1:])]), WIDE[name]
+    kw = dict(kl_coef=0.3, entropy_coef=0.02)
+    near = [100.7, -12345.6, 31000.0]
+    for i, offset in enumerate(near + offsets(dtype)):
+        z, k, _, noise, _, adv, _, valid = far_inputs(heads, dtype, offset, i, N, False)
+        mask = None
+        if masked:                                               # the first choices of some rows: one wave's
+            mask = torch.ones(z.shape, dtype=torch.uint8)
+            mask[2:, 1:4] = 0
+            z = torch.where(mask == 0, torch.tensor(math.nan, dtype=dtype), z)
+        act, logp, entropy, e, e_h = ref.sample(z, heads, noise, mask)
+        old = (logp - 0.05).float()
+        zc, kc, mc, nc, advc, oldc = cuda(z, k, mask, noise, adv, old)
+        got = learning.sample_actions(zc, heads, nc, mc)
+        assert got.actions.cpu().equal(act), offset
+        assert ref.near(got.logp, logp, e) <= 1, offset
+        assert ref.near(got.entropy, entropy, e_h) <= 1, offset
+        for r, v in ((None, valid), (k, None)):
+            want = ref.policy_loss(z, act, adv, old, heads, r, v, mask, **kw)
+            loss = learning.policy_loss_grad(zc, got.actions, advc, oldc, heads, ref_logits=None if r is None else kc,
+                                             valid=None if v is None else v.cuda(), choice_mask=mc, **kw)
+            check_loss(loss, want, dtype)
