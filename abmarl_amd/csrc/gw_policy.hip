@@ -119,6 +119,14 @@ __device__ __forceinline__ float log_of(float x)
     return fmaf(l, LN2, fmaf(x, exp2_of(-l), -1.f));
 }
 
+// v - m of finite logits may pass the largest number; where its exponential is 0, so
+// must be their product.  NaN stays.
+__device__ __forceinline__ float below(float v, float m)
+{
+    const float x = v - m;
+    return x < -1e30f ? -1e30f : x;
+}
+
 template <class T>
 __device__ __forceinline__ float logit_at(const T* row, const uint8_t* mask, int j)
 {
@@ -212,9 +220,9 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
                 for (int j = lo; j < hi; j++) {
                     const float v = logit(j);
                     if (v == NEG_INF) continue;
-                    const float e = expf(v - m);
+                    const float x = below(v, m), e = expf(x);
                     s += e;
-                    t += e * (v - m);
+                    t += e * x;
                 }
                 const float log_s = log_of(s);
                 logp += (at - m) - log_s;
@@ -258,9 +266,9 @@ __global__ __launch_bounds__(G) void sample_rows_kernel(SampleArgs a, Heads h)
             for (int j = lo + tid; j < hi; j += G) {
                 const float v = logit(j);
                 if (v == NEG_INF) continue;
-                const float e = expf(v - m);
+                const float x = below(v, m), e = expf(x);
                 s += e;
-                t += e * (v - m);
+                t += e * x;
             }
             s = grp.sum(s);
             t = grp.sum(t);
@@ -601,7 +609,8 @@ __global__ __launch_bounds__(256) void sample_narrow_kernel(SampleArgs a, Small 
         for (int j = 0; j < CM; j++) {
             const float e = exp_of<T>(v[j]);
             sum += e;
-            t += e * v[j];
+            // (a difference past the largest number: its exponential is 0, not NaN in the product)
+            t += e * fmaxf(v[j], -1e30f);
             // the first of the largest scores; a score of -inf counts for a choice that exists
             const bool better = raw[j] != NEG_INF && (s[j] > best || (choice < 0 && s[j] == best));
             best = better ? s[j] : best;
@@ -1322,13 +1331,13 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                 for (int j = lo; j < hi; j++) {
                     const float v = logit(j);
                     if (v == NEG_INF) continue;
-                    const float e = expf(v - m);
+                    const float x = below(v, m), e = expf(x);
                     s += e;
-                    t += e * (v - m);
+                    t += e * x;
                     if (zr && refs(j) != NEG_INF) {
-                        const float w = refs(j) - mr, er = expf(w);
+                        const float w = below(refs(j), mr), er = expf(w);
                         sr += er;
-                        u += er * (w - (v - m));
+                        u += er * (w - x);
                     }
                 }
                 log_s = log_of(s);
@@ -1366,13 +1375,13 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
                 for (int j = lo + tid; j < hi; j += G) {
                     const float v = logit(j);
                     if (v == NEG_INF) continue;
-                    const float e = expf(v - m);
+                    const float x = below(v, m), e = expf(x);
                     s += e;
-                    t += e * (v - m);
+                    t += e * x;
                     if (zr && refs(j) != NEG_INF) {
-                        const float w = refs(j) - mr, er = expf(w);
+                        const float w = below(refs(j), mr), er = expf(w);
                         sr += er;
-                        u += er * (w - (v - m));
+                        u += er * (w - x);
                     }
                 }
                 s = grp.sum(s);
@@ -1414,7 +1423,7 @@ __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
             const float v = logit(j);
             float gj = 0.f;
             if (v != NEG_INF) {
-                const float x = v - hm[d], p = expf(x) * hinv[d];
+                const float x = below(v, hm[d]), p = expf(x) * hinv[d];
                 // d(-surrogate) pull (1[chosen] - p), KL p - q, entropy p (log p + H)
                 gj = r.pull * ((j - lo == c ? 1.f : 0.f) - p) + a.entropy * p * (x - hls[d] + hh[d]);
                 if (hrinv[d] != 0.f) gj += a.kl * (p - expf(refs(j) - hrm[d]) * hrinv[d]);

@@ -94,3 +94,30 @@ def test_wide_rows_of_any_size(name, masked, dtype):
             loss = learning.policy_loss_grad(zc, got.actions, advc, oldc, heads, ref_logits=None if r is None else kc,
                                              valid=None if v is None else v.cuda(), choice_mask=mc, **kw)
             check_loss(loss, want, dtype)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('name', ['team', 'rtt', 'odd', 'w65', 'w4100', 'w200', 'mixed', 'cells', 'two_wide'])
+def test_differences_past_the_largest_number(name, dtype):
+    """Logits whose difference float32 does not hold: the far ones have
+    probability 0, and nothing is NaN."""
+    heads = LAYOUTS[name]
+    N = 5
+    z = torch.randn(N, heads.n_choices, generator=gen(4)).to(dtype)
+    first = [s.start for s in ref.head_slices(heads)]
+    z[0] = -3e38
+    z[0, first] = 3e38
+    z[1] = -1e38
+    z[1, first] = 3e38
+    z[2] = 3e38
+    z[3] = -3e38
+    act, logp, entropy, e, e_h = ref.sample(z, heads)
+    zc = z.cuda()
+    got = learning.sample_actions(zc, heads)
+    assert got.actions.cpu().equal(act)
+    assert ref.near(got.logp, logp, e) <= 1 and ref.near(got.entropy, entropy, e_h) <= 1
+    adv = torch.randn(N, generator=gen(5))
+    want = ref.policy_loss(z, act, adv, logp.float(), heads, z, kl_coef=0.5, entropy_coef=0.1)
+    got = learning.policy_loss_grad(zc, *cuda(act, adv, logp.float()), heads, ref_logits=zc, kl_coef=0.5, entropy_coef=0.1)
+    check_loss(got, want, dtype)
