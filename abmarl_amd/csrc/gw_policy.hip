@@ -1585,7 +1585,9 @@ struct WideSplit { int v, lanes, threads; };
 bool take_wide(const Heads& h, int size, bool loss, WideSplit* w)
 {
     if (h.n != 1 || h.width <= NARROW) return false;
-    const int pieces = (h.width * size + 15) / 16;
+    const int64_t bytes = (int64_t)h.width * size;      // (2^30 choices are past 32 bits)
+    if (bytes > 16 * 8 * 1024) return false;
+    const int pieces = (int)((bytes + 15) / 16);
     w->v = loss && pieces > 1024 ? 8 : pieces > 16 ? 4 : 1;
     const int lanes = (pieces + w->v - 1) / w->v;
     if (lanes > (w->v == 8 ? 512 : 1024)) return false;
@@ -1710,7 +1712,7 @@ unsigned launch_loss(const LossArgs& a, const Heads& h, hipStream_t st)
         return blocks;
     }
     const unsigned blocks = (unsigned)blocks_for(a.rows);
-    const unsigned stats = 6 * h.n * 4, staged = stats + (a.ref ? 2 : 1) * h.width * 4;
+    const size_t stats = 6 * (size_t)h.n * 4, staged = stats + (a.ref ? 2 : 1) * (size_t)h.width * 4;
     if (h.width >= 8192) hipLaunchKernelGGL((loss_rows_kernel<T, 1024>), dim3(blocks), dim3(1024), stats, st, a, h);
     else if (h.width >= STAGED_ROW) hipLaunchKernelGGL((loss_rows_kernel<T, 256>), dim3(blocks), dim3(256), stats, st, a, h);
     else hipLaunchKernelGGL((loss_rows_kernel<T, 64>), dim3(blocks), dim3(64), staged, st, a, h);

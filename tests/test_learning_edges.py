@@ -121,3 +121,33 @@ def test_differences_past_the_largest_number(name, dtype):
     want = ref.policy_loss(z, act, adv, logp.float(), heads, z, kl_coef=0.5, entropy_coef=0.1)
     got = learning.policy_loss_grad(zc, *cuda(act, adv, logp.float()), heads, ref_logits=zc, kl_coef=0.5, entropy_coef=0.1)
     check_loss(got, want, dtype)
+
+
+@gpu
+@pytest.mark.parametrize('n,dtype', [(1 << 29, torch.float32), (1 << 30, torch.float32), (1 << 30, torch.bfloat16)])
+def test_the_widest_heads(n, dtype):
+    """Rows of 2 and 4 GiB, whose sizes in bytes pass 31 and 32 bits.  All logits are 0 but
+    the last, -3: the sums are n - 1 ones, exact in float32 joined by parts, and e^-3."""
+    heads = PolicyHeads([n])
+    z = torch.zeros((1, n), dtype=dtype, device='cuda')
+    z[0, n - 1] = -3.0
+    total = n - 1 + math.exp(-3)
+    logp, entropy = -math.log(total), math.log(total) + 3 * math.exp(-3) / total
+    room = 16 * 2.0 ** -24 * entropy                             # the joined parts, the logarithm, the result
+    got = learning.sample_actions(z, heads)
+    assert got.actions.item() == 0
+    assert abs(got.logp.item() - logp) <= room and abs(got.entropy.item() - entropy) <= room
+    act = torch.full((1, 1), n - 2, dtype=torch.int32, device='cuda')
+    one = torch.ones(1, device='cuda')
+    g = learning.policy_loss_grad(z, act, one, got.logp, heads, grad_scale=float(n // 2))
+    assert abs(g.logp.item() - logp) <= room and abs(g.loss.item() + 1) <= 2 * room
+    half = torch.finfo(dtype).eps / 2
+    for j, want in ((0, 1 / total), (100, 1 / total), (n // 2, 1 / total), (n - 3, 1 / total), (n - 2, 1 / total - 1),
+                    (n - 1, math.exp(-3) / total)):
+        want *= n // 2
+        assert abs(g.grad[0, j].item() - want) <= abs(want) * (half + 4 * room), j
+    assert int((g.grad > 0).sum()) == n - 1
+    del g
+    z[0, n - 2] = 90.0                                           # the only one left
+    got = learning.sample_actions(z, heads)
+    assert got.actions.item() == n - 2 and got.logp.item() == 0.0
