@@ -831,7 +831,8 @@ __global__ __launch_bounds__(256) void loss_narrow_kernel(LossArgs a, Small h)
             const bool some = sd != 0.f;
             const float inv = some ? rcp_of(sd) : 0.f, log_s = some ? log_of(sd) : 0.f, ts = plane[P_T * WAVE] * inv;
             const Picks of = ((Picks)~(Picks)0 >> (8 * (int)sizeof(Picks) - h.size[d])) << h.first[d];
-            const bool found = (picks & of) != 0 && atd > -1e38f;
+            // (NaN, of a NaN or infinite logit there, is found)
+            const bool found = (picks & of) != 0 && !(atd <= -1e38f);
             entropy += log_s - ts * LN2;
             possible &= found || !some;
             logp += found && some ? (double)(atd * LN2) - (double)log_s : 0.;

@@ -151,3 +151,28 @@ def test_the_widest_heads(n, dtype):
     z[0, n - 2] = 90.0                                           # the only one left
     got = learning.sample_actions(z, heads)
     assert got.actions.item() == n - 2 and got.logp.item() == 0.0
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('bad', [math.nan, math.inf])
+@pytest.mark.parametrize('name', ['team', 'rtt', 'odd', 'w47', 'w65', 'w4100', 'w200', 'cells', 'mixed'])
+def test_a_bad_logit_at_the_chosen_place_shows(name, bad, dtype):
+    """A NaN or +inf logit that was chosen gives NaN in its row's
+    log-probability, policy term and gradient; other rows are as without it."""
+    heads = LAYOUTS[name]
+    N = 5
+    z = torch.randn(N, heads.n_choices, generator=gen(6)).to(dtype)
+    act, logp, _, _, _ = ref.sample(z, heads)
+    args = cuda(act, torch.randn(N, generator=gen(7)), logp.float())
+    kw = dict(entropy_coef=0.0, denominator=1.0)
+    clean = learning.policy_loss_grad(z.cuda(), *args, heads, **kw)
+    s, d = ref.head_slices(heads)[0], heads.slots[0]
+    z[2, s.start + int(act[2, d]) - heads.low[0]] = bad
+    got = learning.policy_loss_grad(z.cuda(), *args, heads, **kw)
+    assert math.isnan(got.logp[2].item()) and math.isnan(got.stats[0].item()) and math.isnan(got.loss.item())
+    assert torch.isnan(got.grad[2].float()).all().item()
+    rest = [0, 1, 3, 4]
+    # a bad row may send its wave another way round: equal within two roundings of the sums
+    assert torch.allclose(got.logp[rest], clean.logp[rest], rtol=0, atol=heads.n_heads * 2.0 ** -20)
+    assert torch.isfinite(got.grad[rest].float()).all().item()
