@@ -353,7 +353,7 @@ def _span(shape, t, name):
     n = 1
     for s in shape[len(lead):]:
         n *= s
-    return n
+    return max(n, 1)                       # (no channels: nothing is read)
 
 
 def _launch_recurrence(gate, value, gate_span, x, state, cut, cut_span, reverse, h, last, carry):
@@ -390,7 +390,9 @@ class _Recurrence(torch.autograd.Function):
         T, device = x.shape[0], x.device
         n = carry.shape[1]
         dx = torch.empty_like(x)
-        dgate = torch.empty_like(gate) if gate is not None and ctx.needs_input_grad[0] else None
+        # (without channels no launch writes the gradient of the gates that they would share)
+        dgate = (torch.empty_like(gate) if n else torch.zeros_like(gate)) \
+            if gate is not None and ctx.needs_input_grad[0] else None
         dstate = torch.empty(x.shape[1:], dtype=torch.float32, device=device) \
             if has_state and ctx.needs_input_grad[2] else None
         dh = None if dh is None else dh.contiguous()

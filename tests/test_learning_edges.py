@@ -176,3 +176,20 @@ def test_a_bad_logit_at_the_chosen_place_shows(name, bad, dtype):
     # a bad row may send its wave another way round: equal within two roundings of the sums
     assert torch.allclose(got.logp[rest], clean.logp[rest], rtol=0, atol=heads.n_heads * 2.0 ** -20)
     assert torch.isfinite(got.grad[rest].float()).all().item()
+
+
+@gpu
+def test_shared_gates_of_no_channels():
+    """A batch of no envs or lanes is no error, and its gates' gradients are 0."""
+    for shape, gshape, cshape in (((5, 0), (5,), (5,)), ((5, 3, 0), (5, 3), (5, 3)), ((5, 0, 4), (5, 0), (5,)),
+                                  ((5, 3, 0), (5, 3, 1), (5, 3, 0))):
+        x = torch.zeros(shape, device='cuda', requires_grad=True)
+        gate = torch.ones(gshape, device='cuda', requires_grad=True)
+        state = torch.zeros(shape[1:], device='cuda', requires_grad=True)
+        cut = torch.zeros(cshape, dtype=torch.uint8, device='cuda')
+        junk = torch.full(gshape, 7.0, device='cuda')            # what freed memory may hold
+        del junk
+        h, last = learning.linear_recurrence(gate, x, state, cut=cut)
+        assert h.shape == shape and last.shape == shape[1:]
+        dg, dx, ds = torch.autograd.grad((h, last), (gate, x, state), (torch.ones_like(h), torch.ones_like(last)))
+        assert dg.shape == gshape and not dg.any().item() and dx.shape == shape and ds.shape == shape[1:]
