@@ -17,6 +17,7 @@ import ctypes as C
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad
 
 from abmarl_amd import _native
 
@@ -176,6 +177,13 @@ def _once():
         raise RuntimeError("the policy operators' gradients cannot be differentiated again (create_graph)")
 
 
+def _no_tangent(*inputs):
+    # (kernels read values only: a tangent would be lost without a word)
+    if forward_ad._current_level >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in inputs):
+        raise NotImplementedError("the policy operators have no forward-mode derivatives")
+
+
 # ------------------------------------------------------------------ sampling
 def sample_actions(logits, heads, noise=None, choice_mask=None, out=None):
     """Draws an action row for each row of logits [..., n_choices] (float32,
@@ -332,6 +340,7 @@ def policy_loss_grad(logits, actions, advantage, old_logp, heads, *, ref_logits=
     args = _loss_args(logits, actions, advantage, old_logp, heads, ref_logits, valid, choice_mask, clip, denominator)
     kl_coef, entropy_coef = _finite('kl_coef', kl_coef), _finite('entropy_coef', entropy_coef)
     grad_scale = _finite('grad_scale', grad_scale)
+    _no_tangent(logits, advantage, old_logp, ref_logits)
     device = logits.device
     _gpu(device)
     loss, stats, logp = _loss_outputs(logits)
@@ -419,8 +428,8 @@ def linear_recurrence(gate, x, state=None, cut=None, reverse=False):
     dropped before the step, as at the first step of an episode (a gate of 0
     drops it too, whatever it holds).
 
-    Differentiable by gate, x and state; a shared gate's gradient is summed
-    in a fixed order.  One step (T = 1) is the form for acting."""
+    Differentiable by gate, x and state (backwards only); a shared gate's gradient
+    is summed in a fixed order.  One step (T = 1) is the form for acting."""
     if not isinstance(x, torch.Tensor) or x.dim() < 2:
         raise ValueError("x: a tensor [steps, ...] is needed")
     _tensor(x, 'x', _FLOATS)
@@ -438,6 +447,7 @@ def linear_recurrence(gate, x, state=None, cut=None, reverse=False):
         _tensor(cut, 'cut', _BYTES, device)
         cut_span = _span(shape, cut, 'cut')
     reverse = int(bool(reverse))
+    _no_tangent(gate, x, state)
     _gpu(device)
     if torch.is_grad_enabled() and (x.requires_grad or (gate is not None and gate.requires_grad) or
                                     (state is not None and state.requires_grad)):

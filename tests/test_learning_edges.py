@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from abmarl_amd import learning
 from abmarl_amd.learning import PolicyHeads
@@ -193,3 +194,19 @@ def test_shared_gates_of_no_channels():
         assert h.shape == shape and last.shape == shape[1:]
         dg, dx, ds = torch.autograd.grad((h, last), (gate, x, state), (torch.ones_like(h), torch.ones_like(last)))
         assert dg.shape == gshape and not dg.any().item() and dx.shape == shape and ds.shape == shape[1:]
+
+
+def test_forward_mode_refused():
+    """A tangent would be lost: the call says so (before it looks for a GPU)."""
+    with fwad.dual_level():
+        x = torch.ones(4, 3)
+        dual = fwad.make_dual(x, x)
+        for args in ((0.5, dual), (dual, x), (0.5, x, fwad.make_dual(x[0], x[0]))):
+            with pytest.raises(NotImplementedError, match='forward'):
+                learning.linear_recurrence(*args)
+        z = torch.zeros(4, 8)
+        rest = torch.zeros(4, 3, dtype=torch.int32), torch.zeros(4), torch.zeros(4), LAYOUTS['team']
+        with pytest.raises(NotImplementedError, match='forward'):
+            learning.policy_loss_grad(fwad.make_dual(z, z), *rest)
+        with pytest.raises(RuntimeError, match='no CPU fallback'):          # no tangent, no complaint
+            learning.policy_loss_grad(z, *rest)
