@@ -362,7 +362,8 @@ class GridWorldEngine:
     def sample_actions(self, logits, noise=None, out=None):
         """Action rows drawn from a policy's logits [..., A, n_choices]
         (learning.sample_actions with policy_heads): for logits [E, A, n] they
-        go into self.actions, which step() takes, unless `out` is given."""
+        go into self.actions, which step() takes, unless `out` is given (the
+        next call's go there too: clone what is kept, or give each its `out`)."""
         heads, mask, _ = self.policy_heads()
         if out is None and logits.shape[:-1] == self.actions.shape[:-1]:
             out = self.actions
