@@ -390,10 +390,25 @@ class GridWorldEngine:
         if 'returned' in out:
             raise ValueError("turn-based slabs: a lane's steps are turns apart, advantages are not defined over them")
         K = int(value.shape[0]) - 1
-        marks = learning.fragment_marks(out['all_done'][:K], start['steps'], horizon, autoreset, start['all_done'],
-                                        self.err)
+        marks = self._fragment_marks(out, K, start, horizon, autoreset)
         return learning.advantages(out['reward'][:K], value, out['done'][:K], marks, start['live'], gamma, lam,
                                    acts=self.policy_heads()[2])
+
+    def _fragment_marks(self, out, K, start, horizon, autoreset):
+        return learning.fragment_marks(out['all_done'][:K], start['steps'], horizon, autoreset, start['all_done'], self.err)
+
+    def linear_recurrence(self, gate, x, out, start, state=None, horizon=0, autoreset='next_step'):
+        """learning.linear_recurrence over a fragment, its state dropped where an
+        env's episode begins: x [K, E, ...] of the observations before each step,
+        or [K + 1, E, ...] with those after the last (as advantages' value);
+        state [E, ...] from before the fragment (its next one's is h of x[K - 1], `last`
+        of K rows); out, start, horizon and autoreset as in advantages()."""
+        if 'returned' in out:
+            raise ValueError("turn-based slabs: a lane's steps are turns apart, its memory is not defined over them")
+        T = int(x.shape[0])
+        marks = self._fragment_marks(out, max(T - 1, 0), start, horizon, autoreset)
+        cut = learning.fragment_cuts(marks, start['steps'])[:T]
+        return learning.linear_recurrence(gate, x, state, cut=cut)
 
     def policy_loss(self, logits, actions, advantage, old_logp, **kw):
         """learning.policy_loss with this engine's heads and lane masks

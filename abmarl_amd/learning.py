@@ -5,10 +5,11 @@ engine's action rows, and from a rollout's slabs to the policy's gradient.
     out = engine.rollout(...)                       # slabs [K][E][A]
     adv = advantages(out['reward'], value, out['done'], marks, live)
     loss = policy_loss(logits, r.actions, adv.advantage, r.logp, heads, valid=adv.valid)
-    h, last = linear_recurrence(gate, x, state, cut=marks)   # a policy's memory
+    cut = fragment_cuts(marks, steps)               # where its memory starts anew
+    h, last = linear_recurrence(gate, x, state, cut=cut[:-1])   # a policy's memory, x [K][E]...
 
-GridWorldEngine has methods of the same names that fill in its own heads,
-lanes and marks.  Tensors stay on the GPU and the calls only put work on the
+GridWorldEngine has sample_actions, advantages, policy_loss, policy_loss_grad and
+linear_recurrence as methods that fill in its own heads, lanes, marks and cuts.  Tensors stay on the GPU and the calls only put work on the
 current stream of the tensors' device: they can be captured into a graph.
 Wrong arguments raise ValueError before anything is launched.  Like the
 engine, the operators have no CPU fallback.
@@ -425,8 +426,9 @@ def linear_recurrence(gate, x, state=None, cut=None, reverse=False):
     gate: like x, or x's first dimensions (channels share a gate; a last
     dimension of 1 may stand for them), of x's dtype or float32; or one number.
     cut: uint8 or bool, x's first dimensions: where it is not 0 the state is
-    dropped before the step, as at the first step of an episode (a gate of 0
-    drops it too, whatever it holds).
+    dropped before the step, as at the first step of an episode (fragment_cuts
+    makes it of a rollout's marks, which stand at an episode's last step; a gate
+    of 0 drops the state too, whatever it holds).
 
     Differentiable by gate, x and state (backwards only); a shared gate's gradient
     is summed in a fixed order.  One step (T = 1) is the form for acting."""
@@ -487,6 +489,30 @@ def fragment_marks(all_done, steps=None, horizon=0, autoreset='next_step', all_d
     _call(_lib().gw_fragment_marks, device, K, E, all_done.data_ptr(), _at(all_done_before), _at(steps), _at(err),
           int(horizon), 1 if autoreset == 'same_step' else 2, marks.data_ptr())
     return marks
+
+
+def fragment_cuts(marks, steps=None):
+    """Where a policy's memory starts anew in a rollout: uint8 [K + 1, E] for the
+    observations before each step and after the last, linear_recurrence's cut for
+    x [K + 1, E, ...] (or cut[:K] for x [K, E, ...]).
+
+    marks: fragment_marks' [K, E].  An observation is an episode's first where the
+    step before it ended one (same_step) or was the reset (next_step).  The memory
+    of an episode that the horizon ended still reaches the observation behind
+    it, whose value advantages() uses; behind an END the reset's own row, which
+    nothing uses, stands alone.  steps: int32 [E], the envs' step counters before
+    the fragment (engine.fragment_start()): 0 where its first observation is an
+    episode's first; None: the state given goes on everywhere."""
+    _tensor(marks, 'marks', (torch.uint8,))
+    _need(marks.dim() == 2, f"marks: shape {tuple(marks.shape)}, not (steps, envs)")
+    K, E = marks.shape
+    if steps is not None:
+        _tensor(steps, 'steps', _I32, marks.device, torch.Size([E]))
+    cut = torch.zeros((K + 1, E), dtype=torch.uint8, device=marks.device)
+    cut[1:] = (marks & (MARK_END | MARK_RESET)) != 0
+    if steps is not None:
+        cut[0] = steps == 0
+    return cut
 
 
 def advantages(reward, value, done, marks, live, gamma=0.99, lam=0.95, acts=None):

@@ -111,7 +111,9 @@ gw_status gw_policy_loss(const gw_policy_heads* heads, int32_t dtype, int64_t n_
      x, h     [n_steps][n] of dtype
      gate     [n_steps][n / gate_span] of gate_dtype (dtype or GW_T_F32): channel
               c uses gate c / gate_span; NULL: gate_value everywhere
-     cut      uint8 [n_steps][n / cut_span] or NULL
+     cut      uint8 [n_steps][n / cut_span] or NULL: set where an episode begins.  (Of a
+              fragment's marks, below: not where END stands but a step behind it, or, where
+              the env is reset by a step of its own, behind RESET)
      state    float [n] or NULL (zeros);  last  float [n]: h after the last
               step done, or NULL
      carry    float [ceil(n_steps / GW_RECURRENCE_SEGMENT)][n] or NULL: h

@@ -9,7 +9,7 @@ import torch.autograd.forward_ad as fwad
 from abmarl_amd import learning
 from abmarl_amd.learning import PolicyHeads
 from tests import learning_reference as ref
-from tests.test_learning import DTYPES, LAYOUTS, check_loss, cuda, gen, gumbel
+from tests.test_learning import DTYPES, LAYOUTS, check_loss, cuda, fragment, gen, gumbel
 
 gpu = pytest.mark.gpu
 
@@ -210,3 +210,36 @@ def test_forward_mode_refused():
             learning.policy_loss_grad(fwad.make_dual(z, z), *rest)
         with pytest.raises(RuntimeError, match='no CPU fallback'):          # no tangent, no complaint
             learning.policy_loss_grad(z, *rest)
+
+
+@pytest.mark.parametrize('mode', ['next_step', 'same_step'])
+def test_memory_is_cut_where_episodes_begin(mode):
+    """Against the envs' own step counters: an observation is an episode's
+    first where no step was taken in it.  The one behind an END, before the
+    reset (next_step), is cut too."""
+    K, E, horizon = 60, 40, 7
+    _, _, _, all_done, before, steps, _, _, _ = fragment(K, E, 2, 3, mode, horizon)
+    marks = ref.marks(all_done, steps, horizon, mode, before)
+    want = torch.zeros((K + 1, E), dtype=torch.uint8)
+    for e in range(E):
+        n, ended = int(steps[e]), bool(before[e])
+        for t in range(K + 1):
+            want[t, e] = n == 0 or (mode == 'next_step' and t > 0 and bool(all_done[t - 1, e]) and not reset)
+            if t == K:
+                break
+            reset = mode == 'next_step' and (ended or n >= horizon)
+            n, ended = (0, False) if reset else (n + 1, bool(all_done[t, e]))
+            if mode == 'same_step' and (ended or n >= horizon):
+                n = 0
+    got = learning.fragment_cuts(marks, steps)
+    assert got.equal(want)
+    assert learning.fragment_cuts(marks)[1:].equal(want[1:]) and not learning.fragment_cuts(marks)[0].any()
+    assert learning.fragment_cuts(marks[:0], steps).equal(want[:1])
+
+
+@pytest.mark.parametrize('kw,word', [
+    (dict(marks=torch.zeros(3, 2)), 'marks'), (dict(marks=torch.zeros(3, dtype=torch.uint8)), 'marks'),
+    (dict(steps=torch.zeros(2)), 'steps'), (dict(steps=torch.zeros(3, dtype=torch.int32)), 'steps')])
+def test_cuts_refused(kw, word):
+    with pytest.raises(ValueError, match=word):
+        learning.fragment_cuts(**{**dict(marks=torch.zeros(3, 2, dtype=torch.uint8)), **kw})
