@@ -9,7 +9,7 @@ import torch.autograd.forward_ad as fwad
 from abmarl_amd import learning
 from abmarl_amd.learning import PolicyHeads
 from tests import learning_reference as ref
-from tests.test_learning import DTYPES, LAYOUTS, check_loss, cuda, fragment, gen, gumbel
+from tests.test_learning import DTYPES, LAYOUTS, _all_calls, check_loss, cuda, fragment, gen, gumbel
 
 gpu = pytest.mark.gpu
 
@@ -243,3 +243,24 @@ def test_memory_is_cut_where_episodes_begin(mode):
 def test_cuts_refused(kw, word):
     with pytest.raises(ValueError, match=word):
         learning.fragment_cuts(**{**dict(marks=torch.zeros(3, 2, dtype=torch.uint8)), **kw})
+
+
+@gpu
+def test_two_streams_at_once_give_their_own_numbers():
+    """Every round's outputs of two streams that run at once, bit for bit."""
+    a, _ = _all_calls(11)
+    b, _ = _all_calls(12)
+    want = [[t.clone() for t in f()] for f in (a, b)]
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    got = [[], []]
+    for _ in range(6):
+        for i, (s, f) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(s):
+                got[i].append(f())
+    torch.cuda.synchronize()
+    for w, rounds in zip(want, got):
+        for out in rounds:
+            assert len(out) == len(w)
+            for x, y in zip(w, out):
+                assert (x == y).logical_or(torch.isnan(x.float()) & torch.isnan(y.float())).all().item()
