@@ -482,13 +482,21 @@ __global__ __launch_bounds__(256) void recur_backward_pair_kernel(RecurArgs a)
 template <class TG>
 __global__ __launch_bounds__(256) void gate_parts_kernel(RecurArgs a)
 {
-    const int64_t gates = a.gates, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= a.T * gates) return;
-    const int64_t lo = i % gates * a.gate_span;
-    const int pieces = (int)((lo + a.gate_span - 1) / WAVE - lo / WAVE) + 1;
-    float s = 0.f;
-    for (int p = 0; p < pieces; p++) s += a.part[i * a.parts + p];
-    ((TG*)a.dgate)[i] = (TG)s;
+    const int64_t gates = a.gates;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.T * gates; i += (int64_t)gridDim.x * 256) {
+        const int64_t lo = i % gates * a.gate_span;
+        const int pieces = (int)((lo + a.gate_span - 1) / WAVE - lo / WAVE) + 1;
+        float s = 0.f;
+        for (int p = 0; p < pieces; p++) s += a.part[i * a.parts + p];
+        ((TG*)a.dgate)[i] = (TG)s;
+    }
+}
+
+// (a launch has fewer than 2^32 threads: beyond 2^30 gates they take several)
+unsigned gate_parts_blocks(const RecurArgs& a)
+{
+    const int64_t need = (a.T * a.gates + 255) / 256;
+    return (unsigned)(need < (1 << 22) ? need : 1 << 22);
 }
 
 __global__ __launch_bounds__(256) void marks_kernel(int64_t T, int64_t E, const uint8_t* all_done,
@@ -720,7 +728,7 @@ void launch_backward(const RecurArgs& a, void* workspace, hipStream_t st)
     else if (q.nw == 4) hipLaunchKernelGGL((recur_backward_kernel<T, TG, 4, 1, SUMS>), grid, dim3(256), 0, st, a, q.s);
     else hipLaunchKernelGGL((recur_backward_kernel<T, TG, 8, 1, SUMS>), grid, dim3(512), 0, st, a, q.s);
     if (SUMS && a.parts > 1)
-        hipLaunchKernelGGL((gate_parts_kernel<TG>), dim3((unsigned)((a.T * a.gates + 255) / 256)), dim3(256), 0,
+        hipLaunchKernelGGL((gate_parts_kernel<TG>), dim3(gate_parts_blocks(a)), dim3(256), 0,
                            st, a);
 }
 
@@ -733,7 +741,7 @@ void launch_backward(const RecurArgs& a, void* workspace, hipStream_t st)
         if (!a.gate || a.gate_span > 1) hipLaunchKernelGGL((recur_backward_pair_kernel<T, TG, true>), blocks, dim3(256), 0, st, b);
         else hipLaunchKernelGGL((recur_backward_pair_kernel<T, TG, false>), blocks, dim3(256), 0, st, b);
         if (b.dgate && a.gate_span > 1 && b.parts > 1)
-            hipLaunchKernelGGL((gate_parts_kernel<TG>), dim3((unsigned)((b.T * b.gates + 255) / 256)), dim3(256), 0, st, b);
+            hipLaunchKernelGGL((gate_parts_kernel<TG>), dim3(gate_parts_blocks(b)), dim3(256), 0, st, b);
         return;
     }
     if (a.dgate && a.gate_span > 1) launch_backward<T, TG, true>(a, workspace, st);
