@@ -301,7 +301,8 @@ __device__ __forceinline__ RowLoss row_loss(const LossArgs& a, float adv, float 
     r.logp = possible ? (float)logp : NEG_INF;
     const float ratio = possible ? expf((float)(logp - (double)old)) : 0.f;
     const float clamped = fminf(fmaxf(ratio, a.lo), a.hi);
-    const float free = ratio * adv, held = (ratio != ratio ? ratio : clamped) * adv;
+    // (a ratio past the largest number is no NaN beside an advantage of 0)
+    const float free = ratio == -NEG_INF && adv == 0.f ? 0.f : ratio * adv, held = (ratio != ratio ? ratio : clamped) * adv;
     r.clipped = held < free;
     r.pull = r.clipped ? 0.f : -free;
     r.pg = r.clipped ? -held : -free;

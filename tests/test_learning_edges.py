@@ -287,3 +287,21 @@ def test_two_to_the_32_shared_gates():
     assert not (dg[:-tail] != 0).any().item()
     del x, gate, last, dg
     torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize('name', ['team', 'rtt', 'w65', 'w4100', 'cells'])
+def test_no_advantage_beside_a_ratio_past_the_largest_number(name):
+    """A row without an advantage has no policy term, however far its action's
+    probability has risen; with one, the clipped term."""
+    heads = LAYOUTS[name]
+    N = 6
+    z = torch.randn(N, heads.n_choices, generator=gen(9))
+    act, logp, _, _, _ = ref.sample(z, heads)
+    old = (logp - torch.tensor([200.0, 0.05, 5.0, 300.0, 0.0, 89.0])).float()
+    adv = torch.tensor([0.0, 1.0, 2.0, 0.0, 0.0, 0.0])
+    want = ref.policy_loss(z, act, adv, old, heads, entropy_coef=0.1)
+    args = cuda(act, adv, old)
+    check_loss(learning.policy_loss_grad(z.cuda(), *args, heads, entropy_coef=0.1), want, torch.float32)
+    old[0] = old[3] = -math.inf                                  # impossible before, now drawn
+    check_loss(learning.policy_loss_grad(z.cuda(), *cuda(act, adv, old), heads, entropy_coef=0.1), want, torch.float32)
