@@ -237,14 +237,14 @@ def _loss_args(logits, actions, advantage, old_logp, heads, ref_logits, valid, c
     mask, mask_rows = _mask(choice_mask, logits.shape, device)
     low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
     low, high = float(low), float(high)
-    if not (0 <= low < _INF and 0 <= high < _INF):
-        raise ValueError(f"clip {clip}: finite, not negative")
+    if not (0 <= low and C.c_float(low).value < _INF and 0 <= high and C.c_float(high).value < _INF):
+        raise ValueError(f"clip {clip}: finite in float32, not negative")
     value, at = 0.0, None
     if isinstance(denominator, torch.Tensor):
         at = _tensor(denominator, 'denominator', _F32, device, torch.Size([]))
     elif denominator is not None:
-        value = float(denominator)
-        _need(0 < value < float('inf'), f"denominator {denominator}: finite and positive")
+        value = C.c_float(float(denominator)).value
+        _need(0 < value < _INF, f"denominator {denominator}: finite and positive in float32")
     if advantage.requires_grad or old_logp.requires_grad or ref_logits is not None and ref_logits.requires_grad:
         raise ValueError("advantage, old_logp, ref_logits: no gradient flows to them, detach them")
     return n, ld, ld_ref, mask, mask_rows, low, high, value, at
@@ -252,8 +252,8 @@ def _loss_args(logits, actions, advantage, old_logp, heads, ref_logits, valid, c
 
 def _finite(name, v):
     v = float(v)
-    if not abs(v) < _INF:
-        raise ValueError(f"{name} {v}: must be finite")
+    if not abs(C.c_float(v).value) < _INF:               # (as the kernels take it)
+        raise ValueError(f"{name} {v}: must be finite in float32")
     return v
 
 

@@ -305,3 +305,17 @@ def test_no_advantage_beside_a_ratio_past_the_largest_number(name):
     check_loss(learning.policy_loss_grad(z.cuda(), *args, heads, entropy_coef=0.1), want, torch.float32)
     old[0] = old[3] = -math.inf                                  # impossible before, now drawn
     check_loss(learning.policy_loss_grad(z.cuda(), *cuda(act, adv, old), heads, entropy_coef=0.1), want, torch.float32)
+
+
+@pytest.mark.parametrize('change,word', [
+    (dict(denominator=1e-60), 'denominator'), (dict(denominator=1e39), 'denominator'), (dict(kl_coef=1e39), 'kl_coef'),
+    (dict(entropy_coef=-1e39), 'entropy_coef'), (dict(clip=1e39), 'clip'), (dict(clip=(0.2, 1e300)), 'clip')])
+def test_numbers_that_float32_does_not_hold_are_refused(change, word):
+    """A denominator that float32 rounds to 0 would have been the number of
+    valid rows in its place."""
+    args = (torch.zeros(4, 8), torch.zeros(4, 3, dtype=torch.int32), torch.zeros(4), torch.zeros(4), LAYOUTS['team'])
+    for fn in (learning.policy_loss, learning.policy_loss_grad):
+        with pytest.raises(ValueError, match=word):
+            fn(*args, **change)
+    with pytest.raises(ValueError, match='gate'):
+        learning.linear_recurrence(1e39, torch.zeros(3, 2))
