@@ -1521,6 +1521,7 @@ gw_status take_heads(const gw_policy_heads* p, Heads* h)
         LEARN_NEED(p->slots[d] >= 0 && p->slots[d] < p->act_dim, "head %d: column %d outside 0..%d", d,
                    p->slots[d], p->act_dim - 1);
         for (int e = 0; e < d; e++) LEARN_NEED(p->slots[e] != p->slots[d], "heads %d and %d share column %d", e, d, p->slots[d]);
+        LEARN_NEED((int64_t)p->low[d] + p->sizes[d] <= (INT64_C(1) << 31), "head %d: values from %d pass int32", d, p->low[d]);
         h->off[d] = (int32_t)w;
         h->low[d] = p->low[d];
         h->slot[d] = (int16_t)p->slots[d];

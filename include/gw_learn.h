@@ -50,7 +50,7 @@ typedef struct gw_policy_heads {
     int32_t n_heads;               /* 1..GW_MAX_HEADS                        */
     int32_t act_dim;               /* >= 1                                   */
     const int32_t* sizes;          /* >= 1 each                              */
-    const int32_t* low;
+    const int32_t* low;            /* low[d] + sizes[d] <= 2^31              */
     const int32_t* slots;          /* 0..act_dim-1, each at most once        */
 } gw_policy_heads;
 

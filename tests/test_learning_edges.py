@@ -1,12 +1,13 @@
 """The policy operators at the ends of their range, against the same 64-bit
 definitions and counted bounds."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 
-from abmarl_amd import learning
+from abmarl_amd import _native, learning
 from abmarl_amd.learning import PolicyHeads
 from tests import learning_reference as ref
 from tests.test_learning import DTYPES, LAYOUTS, _all_calls, _gradients, check_loss, cuda, fragment, gen, gumbel
@@ -319,3 +320,14 @@ def test_numbers_that_float32_does_not_hold_are_refused(change, word):
             fn(*args, **change)
     with pytest.raises(ValueError, match='gate'):
         learning.linear_recurrence(1e39, torch.zeros(3, 2))
+
+
+def test_c_entry_refuses_values_past_int32():
+    """Heads whose values an int32 action does not hold, given past PolicyHeads' own check."""
+    _native.build_learn()
+    L = _native.learn_lib()
+    one = C.c_void_p(8)
+    ints = C.c_int32 * 2
+    heads = learning._Heads(2, 2, ints(3, 5), ints(0, 2 ** 31 - 4), ints(0, 1))
+    args = C.addressof(heads), 0, 4, one, 8, None, None, 0, one, None, None, None
+    assert L.gw_policy_sample(*args) == -1 and b'int32' in L.gw_learn_last_error()
