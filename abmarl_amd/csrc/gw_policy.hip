@@ -428,7 +428,7 @@ __device__ __forceinline__ void block_sums(const LossArgs& a, double* s)
 // Large calls are bound by the vector units and by waits between a tile's loads
 // and its sums, with the registers a row takes for a limit on waves:
 //   5.2 M rows of 3, 3, 2 bf16, ref and valid flags, loss and gradient: 147 us,
-//     382 MB at 2.6 TB/s (a copy: 5.2); about 85 us of it are arithmetic;
+//     382 MB at 2.6 TB/s (a copy: 5.2); 87 lane instructions a choice, about 93 us of issue;
 //   1.0 M rows of 28 choices f16, masks of 256 lanes: loss 65 us, gradient 95 us;
 //   262144 rows of 3, 3, 2 bf16 drawn with their noise: 8.2 us, 17.6 MB (3.4 us).
 // Forcing more waves a CU by launch bounds spilt registers and was slower.
@@ -1280,8 +1280,8 @@ __global__ __launch_bounds__(L ? 256 : V == 8 ? 512 : 1024) void loss_wide_kerne
 }
 
 // One row by one workgroup of G threads, as sample_rows_kernel: maximum,
-// sums, gradient are three walks over a head (512 rows of 40000 float32, which no
-// group's registers hold: 210 us).
+// sums, gradient are three walks over a head (512 rows of 40000 float32 with ref, which
+// no group's registers hold: 214 us; drawing them, two walks and the noise: 103 us).
 template <class T, int G>
 __global__ __launch_bounds__(G) void loss_rows_kernel(LossArgs a, Heads h)
 {
@@ -1580,7 +1580,7 @@ void launch_sample_narrow(const SampleArgs& a, const Small& s, hipStream_t st)
 // wave's lanes in one (65536 rows of 300 bf16, loss and gradient with ref: 64 us, 94
 // us with one piece a lane; of 65 f32, 17 pieces: 30 and 38).  Above 1024 pieces the loss
 // takes eight a lane: fewer waves a row hold fewer copies of what is not the
-// row, so three rows fit a CU in place of two (4099 x 12800 bf16: 119 us, 130 us
+// row, so three rows fit a CU in place of two (4099 x 12800 bf16: 8% less time than
 // with four; drawing 1024 of them f16, one row and its noise, takes 27 us with eight
 // and 24 with four).
 struct WideSplit { int v, lanes, threads; };

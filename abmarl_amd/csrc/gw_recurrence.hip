@@ -36,7 +36,7 @@ struct RecurArgs {
 //   65537 steps of 96 channels f32, a gate a step: maps 12 and 12 us, walks 19 and
 //     28 us, parts of the gates' sums 4 us, where 127 MB would take 24 us: a
 //     chunk's 8 waves wait for each other's maps, and for those of the chunks before;
-//   one step of 262144 channels bf16: 7.0 us, a launch and one round trip.
+//   one step of 262144 channels bf16: 6.9 us, a launch and one round trip.
 
 struct Map { float a, b; };
 

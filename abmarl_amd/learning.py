@@ -314,8 +314,8 @@ def policy_loss(logits, actions, advantage, old_logp, heads, *, ref_logits=None,
     logits, ref_logits: [..., n_choices] float32, float16 or bfloat16, rows one stride
     apart; ref_logits None: no KL.  actions: int32 [..., act_dim] as
     sample_actions gives them.  advantage, old_logp: float32 [...].  valid: uint8 or
-    bool [...]: rows with 0 (agents that did not act) are not read and get no
-    gradient.  choice_mask: as sample_actions'.  clip: one number, or the lower
+    bool [...]: rows with 0 (agents that did not act) count for nothing, whatever
+    stands in them, and get no gradient.  choice_mask: as sample_actions'.  clip: one number, or the lower
     and the upper.  denominator: what to divide by instead of the number of
     valid rows (a number or a float32 device scalar, e.g. all ranks' rows).
     An action whose choice there is not has probability 0: logp -inf, ratio 0.

@@ -90,7 +90,8 @@ gw_status gw_policy_sample(const gw_policy_heads* heads, int32_t dtype, int64_t 
      ref      NULL: no KL term.  valid: NULL: every row
    An action outside its head, or whose choice does not exist, has
    probability 0: L = -inf, ratio 0, no gradient from the policy term.
-   Rows not valid are not read.  The sums over rows are made in double in a
+   What stands in rows not valid is never used (NaN, infinities and any action
+   included), but it may be read.  The sums over rows are made in double in a
    fixed order: the same inputs give the same bits.
    workspace: gw_policy_loss_workspace(n_rows) bytes, 8-byte aligned, free
    for other use once the call's work is done.                              */
