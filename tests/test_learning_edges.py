@@ -331,3 +331,32 @@ def test_c_entry_refuses_values_past_int32():
     heads = learning._Heads(2, 2, ints(3, 5), ints(0, 2 ** 31 - 4), ints(0, 1))
     args = C.addressof(heads), 0, 4, one, 8, None, None, 0, one, None, None, None
     assert L.gw_policy_sample(*args) == -1 and b'int32' in L.gw_learn_last_error()
+
+
+@gpu
+@pytest.mark.parametrize('name', ['team', 'rtt', 'w65', 'w300', 'w4100', 'cells'])
+def test_ref_of_another_size_than_the_logits(name):
+    """KL does not change when all of ref's logits, or all of the policy's, move together."""
+    heads = LAYOUTS[name]
+    N = 40 if heads.n_choices < 400 else 5
+    z0, k0 = (8 * torch.randn(N, heads.n_choices, generator=gen(i)).round() for i in (1, 2))
+    act = ref.sample(z0, heads)[0]
+    adv, valid = torch.randn(N, generator=gen(3)), (torch.rand(N, generator=gen(4)) < 0.7).to(torch.uint8)
+    for dz, dk in ((0.0, 2.0 ** 26), (-2.0 ** 26, 0.0), (2.0 ** 14, -2.0 ** 26), (2.0 ** 26, 2.0 ** 26)):
+        z, k = z0 + dz, k0 + dk                                  # (steps of 8: exact)
+        want = ref.policy_loss(z, act, adv, torch.full((N,), -3.0), heads, k, valid, kl_coef=0.3, entropy_coef=0.02)
+        got = learning.policy_loss_grad(*cuda(z, act, adv), torch.full((N,), -3.0).cuda(), heads, ref_logits=k.cuda(),
+                                        valid=valid.cuda(), kl_coef=0.3, entropy_coef=0.02)
+        # the bounds count |logits - ref| beside each other: here of the rows as they were
+        near = ref.policy_loss(z0, act, adv, torch.full((N,), -3.0), heads, k0, valid, kl_coef=0.3, entropy_coef=0.02)
+        assert abs(near['loss'] - want['loss']) <= 1e-9 * (1 + abs(near['loss']))
+        check_loss(got, near, torch.float32)
+
+
+@gpu
+def test_policy_loss_refuses_forward_mode():
+    with fwad.dual_level():
+        z = torch.zeros(4, 8, device='cuda')
+        rest = torch.zeros(4, 3, dtype=torch.int32).cuda(), torch.zeros(4).cuda(), torch.zeros(4).cuda(), LAYOUTS['team']
+        with pytest.raises(NotImplementedError):
+            learning.policy_loss(fwad.make_dual(z, z), *rest)
